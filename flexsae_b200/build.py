@@ -24,8 +24,11 @@ INCLUDE = os.path.join(os.path.dirname(PKG), "include")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-std=c++17", "-lineinfo",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC",
 ]
+#: sources compiled without ``--use_fast_math``: the optimizer's 8-bit states are rounded on bit patterns
+#: that flush-to-zero would destroy, and its 32-bit update uses IEEE division and square root
+IEEE_SOURCES = ("flexsae_optim.cu",)
 
 
 def _sources():
@@ -53,14 +56,32 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
     if trace:
         extra = extra + ["-DFLEXSAE_TRACE"]
     tmp = f"{out}.{os.getpid()}.tmp"
-    cmd = [nvcc] + NVCC_FLAGS + extra + (["-Xptxas", "-v"] if verbose else []) + ["-I", INCLUDE, "-o", tmp] + _sources()
-    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
-    if verbose or res.returncode != 0:
-        sys.stderr.write(res.stdout)
-    if res.returncode != 0:
+    objects, log = [], ""
+    try:
+        running = []
+        for src in _sources():                          # one compiler per source, side by side
+            name = os.path.basename(src)
+            flags = [f for f in extra if not (name in IEEE_SOURCES and f == "--use_fast_math")]
+            obj = f"{tmp}.{name}.o"
+            objects.append(obj)
+            cmd = [nvcc] + NVCC_FLAGS + flags + (["-Xptxas", "-v"] if verbose else []) + ["-I", INCLUDE, "-c", "-o", obj, src]
+            running.append(subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True))
+        done = [(p.communicate()[0], p.returncode) for p in running]
+        log, failed = "".join(text for text, _ in done), any(rc for _, rc in done)
+        if not failed:
+            res = subprocess.run([nvcc] + NVCC_FLAGS + ["-shared", "-o", tmp] + objects, stdout=subprocess.PIPE,
+                                 stderr=subprocess.STDOUT, text=True)
+            log, failed = log + res.stdout, res.returncode != 0
+    finally:
+        for obj in objects:
+            if os.path.exists(obj):
+                os.remove(obj)
+    if verbose or failed:
+        sys.stderr.write(log)
+    if failed:
         if os.path.exists(tmp):
             os.remove(tmp)
-        raise RuntimeError("nvcc failed:\n" + res.stdout[-4000:])
+        raise RuntimeError("nvcc failed:\n" + log[-4000:])
     os.replace(tmp, out)    # a reader (another rank, a running job) never sees a half-written library
     return out
 

@@ -26,6 +26,7 @@
 
 #include "flexsae_common.cuh"
 #include "flexsae_deterministic.cuh"
+#include "flexsae_host.cuh"
 #include "flexsae_kernel_args.cuh"
 
 namespace flexsae {
@@ -55,9 +56,9 @@ struct Options {
 static Options g_opt;
 
 static thread_local char t_err[512] = "";
-static thread_local int t_launches = 0;
+thread_local int t_launches = 0;
 
-static int fail(int code, const char* fmt, ...) {
+int fail(int code, const char* fmt, ...) {
   va_list ap;
   va_start(ap, fmt);
   vsnprintf(t_err, sizeof(t_err), fmt, ap);

@@ -1,0 +1,705 @@
+// The optimizer step behind the decoder losses: norm of all gradients, AdamW with 32-bit or 8-bit
+// states over a list of tensors, AdamW on a decoder whose rows are kept at unit length.  The
+// reference stops at the gradients (torch-ext/flex_sae/hierarchical_kernels.py:288-299).
+//
+// Every operator is one pass over its data, bound by HBM: per parameter the step reads the parameter,
+// its gradient and two states and writes three of them back (22 bytes with 16-bit weights and 32-bit
+// states, 10 bytes with 8-bit states).
+#include <algorithm>
+#include <math.h>
+#include <new>
+
+#include "flexsae_optim.cuh"
+
+namespace flexsae {
+
+// ---- gradient norm --------------------------------------------------------------------------------------
+constexpr int kNormUnits = 4;                               // units of 256 elements a warp takes at a time
+constexpr int kNormChunk = kOptChunk * kNormUnits;
+constexpr int kNormGrid = 148 * 8;
+
+template <int N>
+struct NormBatch {
+  double* partial;            // one sum per CTA
+  unsigned chunks;
+  int count;
+  unsigned first[N + 1];
+  const void* grad[N];
+  long long numel[N];
+  unsigned char dtype[N], vec[N];
+};
+
+// Sum of eight squares.  The plain 32-bit sum is used where it neither overflowed nor lost terms to
+// underflow; otherwise the squares are formed in 64 bits, so that a norm is finite whenever the
+// result fits the output.
+__device__ __forceinline__ double sum_squares(const float* x) {
+  float s = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; j++) s = fmaf(x[j], x[j], s);
+  if (s >= 0x1p-90f && s <= FLT_MAX) return (double)s;
+  unsigned any = 0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) any |= __float_as_uint(x[j]) << 1;
+  if (!any) return 0.0;
+  double d = 0.0;
+#pragma unroll
+  for (int j = 0; j < 8; j++) d = fma((double)x[j], (double)x[j], d);
+  return d;
+}
+
+__device__ __forceinline__ double block_sum(double v) {
+  __shared__ double part[kOptThreads / 32];
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+  __syncthreads();
+  v = 0.0;
+  for (int i = 0; i < kOptThreads / 32; i++) v += part[i];
+  return v;
+}
+
+template <typename T>
+__device__ __forceinline__ double norm_chunk(const void* grad, long long e0, long long numel, bool aligned, int lane) {
+  double acc = 0.0;
+  if (aligned && e0 + kNormUnits * kOptBlock <= numel) {
+    float x[kNormUnits][8];
+#pragma unroll
+    for (int u = 0; u < kNormUnits; u++) opt_load<T>(grad, e0 + u * kOptBlock, numel, true, lane, 32, x[u]);
+#pragma unroll
+    for (int u = 0; u < kNormUnits; u++) acc += sum_squares(x[u]);
+  } else {
+    for (int u = 0; u < kNormUnits; u++) {
+      float x[8];
+      opt_load<T>(grad, e0 + u * kOptBlock, numel, false, lane, 32, x);
+      acc += sum_squares(x);
+    }
+  }
+  return acc;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_constant__ NormBatch<N> b) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double acc = 0.0;
+  int i = 0;
+  for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    while (c >= b.first[i + 1]) i++;
+    const long long e0 = (long long)(c - b.first[i]) * kNormChunk + warp * (kNormUnits * kOptBlock);
+    if (e0 >= b.numel[i]) continue;
+    if (b.dtype[i] == FLEXSAE_F32)
+      acc += norm_chunk<float>(b.grad[i], e0, b.numel[i], b.vec[i], lane);
+    else if (b.dtype[i] == FLEXSAE_BF16)
+      acc += norm_chunk<__nv_bfloat16>(b.grad[i], e0, b.numel[i], b.vec[i], lane);
+    else
+      acc += norm_chunk<__half>(b.grad[i], e0, b.numel[i], b.vec[i], lane);
+  }
+  acc = block_sum(acc);
+  if (threadIdx.x == 0) b.partial[blockIdx.x] = acc;
+}
+
+__global__ void __launch_bounds__(kOptThreads) grad_norm_finish_kernel(const double* partial, int n, float* out) {
+  double acc = 0.0;
+  for (int i = threadIdx.x; i < n; i += kOptThreads) acc += partial[i];
+  acc = block_sum(acc);
+  if (threadIdx.x == 0) *out = (float)sqrt(acc);
+}
+
+// ---- AdamW, 32-bit states -----------------------------------------------------------------------------
+__device__ __forceinline__ float adamw_param(const OptScalars& s, const OptCoefs& c, float p, float m, float v) {
+  return p * c.decay - c.rate * (m / (sqrtf(v) * c.root + s.eps));
+}
+
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kOptThreads) adamw_kernel(const __grid_constant__ OptBatch<N> b) {
+  OptCoefs co;
+  if (!opt_coefs(b.s, co)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int i = 0;
+  for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    i = opt_find<N>(b, c, i);
+    const OptTensor& t = b.t[i];
+    const long long e0 = (long long)(c - b.first[i]) * kOptChunk + warp * kOptBlock;
+    if (e0 >= t.numel) continue;
+    const bool vec = t.vec && e0 + kOptBlock <= t.numel;
+    float p[8], g[8], m[8], v[8];
+    if (MASTER)
+      opt_load<float>(t.master, e0, t.numel, vec, lane, 32, p);
+    else
+      opt_load<P>(t.param, e0, t.numel, vec, lane, 32, p);
+    opt_load<G>(t.grad, e0, t.numel, vec, lane, 32, g);
+    opt_load<float>(t.exp_avg, e0, t.numel, vec, lane, 32, m);
+    opt_load<float>(t.exp_avg_sq, e0, t.numel, vec, lane, 32, v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      opt_moments(b.s, __fmul_rn(g[j], co.clip), m[j], v[j]);
+      p[j] = adamw_param(b.s, co, p[j], m[j], v[j]);
+    }
+    opt_store<P>(t.param, e0, t.numel, vec, lane, 32, p);
+    if (MASTER) opt_store<float>(t.master, e0, t.numel, vec, lane, 32, p);
+    opt_store<float>(t.exp_avg, e0, t.numel, vec, lane, 32, m);
+    opt_store<float>(t.exp_avg_sq, e0, t.numel, vec, lane, 32, v);
+  }
+  opt_advance(b.s, co.t);
+}
+
+// ---- AdamW, 8-bit states --------------------------------------------------------------------------------
+// m is held as e4m3 and v as e5m2, each times one 32-bit scale per 256 elements.  Both are rounded at
+// random between their two neighbours: with b2 = 0.999 a step changes v by about 0.1 %, far less than
+// half the spacing of an 8-bit float, so that rounding to nearest would never move it; rounding upwards
+// with the probability (v - lower) / (upper - lower) keeps the average right.  Adding random bits
+// below the last kept one and cutting off does exactly that on the bit pattern of a 32-bit float whose
+// exponent has been moved to the small format's, subnormals included (they become 32-bit subnormals).
+constexpr float kScaleM = (float)((1.0 / 448.0) * (1.0 + 0x1p-20));     // the largest value stays below the format's last
+constexpr float kScaleV = (float)((1.0 / 57344.0) * (1.0 + 0x1p-20));
+
+__device__ __forceinline__ unsigned code_e4m3(float x, float inverse, unsigned random20) {
+  const unsigned b = __float_as_uint(__fmul_rn(__fmul_rn(x, inverse), 0x1p-120f));
+  return (((b & 0x7fffffffu) + random20) >> 20) | ((b >> 24) & 0x80u);
+}
+
+// v never becomes zero beside larger values: it is at least the format's smallest number (2^-32 of the
+// block's largest value), so an element is not divided by its eps alone because its neighbours are large.
+__device__ __forceinline__ unsigned code_e5m2(float x, float inverse, unsigned random21) {
+  const float y = fmaxf(__fmul_rn(__fmul_rn(x, inverse), 0x1p-112f), __uint_as_float(0x00200000u));
+  return (__float_as_uint(y) + random21) >> 21;
+}
+
+__device__ __forceinline__ float scale_of(unsigned largest, float factor) {
+  const float s = __fmul_rn(__uint_as_float(largest), factor);
+  return s >= FLT_MIN ? s : 0.0f;
+}
+
+__device__ __forceinline__ float2 widen_fp8x2(unsigned two, __nv_fp8_interpretation_t kind) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, kind)));
+}
+
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kOptThreads) adamw8_kernel(const __grid_constant__ OptBatch<N> b) {
+  OptCoefs co;
+  if (!opt_coefs(b.s, co)) return;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int i = 0;
+  for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+    i = opt_find<N>(b, c, i);
+    const OptTensor& t = b.t[i];
+    const long long e0 = (long long)(c - b.first[i]) * kOptChunk + warp * kOptBlock;
+    if (e0 >= t.numel) continue;      // the same for the whole warp
+    const bool vec = t.vec && e0 + kOptBlock <= t.numel;
+    const long long blk = e0 / kOptBlock;
+    const unsigned key = opt_key(b.s.seed, co.t, t.index);
+    float p[8], g[8], m[8], v[8];
+    if (MASTER)
+      opt_load<float>(t.master, e0, t.numel, vec, lane, 32, p);
+    else
+      opt_load<P>(t.param, e0, t.numel, vec, lane, 32, p);
+    opt_load<G>(t.grad, e0, t.numel, vec, lane, 32, g);
+    const float sm = t.exp_avg_scale[blk], sv = t.exp_avg_sq_scale[blk];
+    unsigned char* m8 = reinterpret_cast<unsigned char*>(t.exp_avg);
+    unsigned char* v8 = reinterpret_cast<unsigned char*>(t.exp_avg_sq);
+    if (vec) {
+      const uint2 cm = *reinterpret_cast<const uint2*>(m8 + e0 + lane * 8);
+      const uint2 cv = *reinterpret_cast<const uint2*>(v8 + e0 + lane * 8);
+#pragma unroll
+      for (int j = 0; j < 8; j += 2) {
+        const float2 a = widen_fp8x2((j < 4 ? cm.x : cm.y) >> (j & 2) * 8 & 0xffffu, __NV_E4M3);
+        const float2 q = widen_fp8x2((j < 4 ? cv.x : cv.y) >> (j & 2) * 8 & 0xffffu, __NV_E5M2);
+        m[j] = a.x, m[j + 1] = a.y, v[j] = q.x, v[j + 1] = q.y;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const long long e = e0 + j * 32 + lane;
+        m[j] = e < t.numel ? widen_fp8x2(m8[e], __NV_E4M3).x : 0.0f;
+        v[j] = e < t.numel ? widen_fp8x2(v8[e], __NV_E5M2).x : 0.0f;
+      }
+    }
+    unsigned top_m = 0, top_v = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      m[j] = __fmul_rn(m[j], sm);
+      v[j] = __fmul_rn(v[j], sv);
+      opt_moments(b.s, __fmul_rn(g[j], co.clip), m[j], v[j]);
+      p[j] = adamw_param(b.s, co, p[j], m[j], v[j]);
+      top_m = max(top_m, __float_as_uint(m[j]) & 0x7fffffffu);
+      top_v = max(top_v, __float_as_uint(v[j]) & 0x7fffffffu);
+    }
+    opt_store<P>(t.param, e0, t.numel, vec, lane, 32, p);
+    if (MASTER) opt_store<float>(t.master, e0, t.numel, vec, lane, 32, p);
+    top_m = __reduce_max_sync(0xffffffffu, top_m);
+    top_v = __reduce_max_sync(0xffffffffu, top_v);
+    const bool odd_values = max(top_m, top_v) >= 0x7f800000u;
+    if (odd_values) {                 // infinities and NaN keep to their own elements: the scale is that of the others
+      top_m = top_v = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const unsigned bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
+        if (bm < 0x7f800000u) top_m = max(top_m, bm);
+        if (bv < 0x7f800000u) top_v = max(top_v, bv);
+      }
+      top_m = __reduce_max_sync(0xffffffffu, top_m);
+      top_v = __reduce_max_sync(0xffffffffu, top_v);
+    }
+    const float new_sm = scale_of(top_m, kScaleM), new_sv = scale_of(top_v, kScaleV);
+    const float im = new_sm > 0.0f ? __frcp_rn(new_sm) : 0.0f, iv = new_sv > 0.0f ? __frcp_rn(new_sv) : 0.0f;
+    unsigned qm[8], qv[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const long long e = vec ? e0 + lane * 8 + j : e0 + j * 32 + lane;
+      const unsigned h = opt_mix((unsigned)(e >> 1) ^ (key + (unsigned)(e >> 33)));
+      qm[j] = code_e4m3(m[j], im, e & 1 ? h & 0xfffffu : h >> 12);
+      qv[j] = code_e5m2(v[j], iv, e & 1 ? h >> 11 : h & 0x1fffffu);
+      if (odd_values) {
+        if ((__float_as_uint(m[j]) & 0x7fffffffu) >= 0x7f800000u) qm[j] = 0x7f;
+        if ((__float_as_uint(v[j]) & 0x7fffffffu) >= 0x7f800000u) qv[j] = 0x7f;
+      }
+    }
+    if (vec) {
+      *reinterpret_cast<uint2*>(m8 + e0 + lane * 8) =
+          make_uint2(qm[0] | qm[1] << 8 | qm[2] << 16 | qm[3] << 24, qm[4] | qm[5] << 8 | qm[6] << 16 | qm[7] << 24);
+      *reinterpret_cast<uint2*>(v8 + e0 + lane * 8) =
+          make_uint2(qv[0] | qv[1] << 8 | qv[2] << 16 | qv[3] << 24, qv[4] | qv[5] << 8 | qv[6] << 16 | qv[7] << 24);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        const long long e = e0 + j * 32 + lane;
+        if (e < t.numel) {
+          m8[e] = (unsigned char)qm[j];
+          v8[e] = (unsigned char)qv[j];
+        }
+      }
+    }
+    if (lane == 0) {
+      t.exp_avg_scale[blk] = new_sm;
+      t.exp_avg_sq_scale[blk] = new_sv;
+    }
+  }
+  opt_advance(b.s, co.t);
+}
+
+// ---- AdamW on a decoder with unit rows --------------------------------------------------------------------
+struct RowArgs {
+  OptScalars s;
+  OptTensor t;
+  long long rows;
+  int cols;
+};
+
+// Sums of two values over the CTA.  `part` is not written again before every thread has passed another barrier.
+__device__ __forceinline__ float2 cta_sum2(float a, float b, float2* part, int warps) {
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, m);
+    b += __shfl_xor_sync(0xffffffffu, b, m);
+  }
+  if (warps == 1) return make_float2(a, b);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) part[threadIdx.x >> 5] = make_float2(a, b);
+  __syncthreads();
+  const float2 q = lane < warps ? part[lane] : make_float2(0.0f, 0.0f);
+  a = q.x, b = q.y;
+#pragma unroll
+  for (int m = 16; m > 0; m >>= 1) {
+    a += __shfl_xor_sync(0xffffffffu, a, m);
+    b += __shfl_xor_sync(0xffffffffu, b, m);
+  }
+  return make_float2(a, b);
+}
+
+// One CTA per row at a time, eight elements per thread, so the row stays in registers between the
+// projection, the step and the division by its length.
+template <typename P, typename G, bool MASTER>
+__global__ void __launch_bounds__(1024) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
+  OptCoefs co;
+  if (!opt_coefs(a.s, co)) return;
+  __shared__ float2 part[2][32];
+  const int warps = blockDim.x >> 5, lanes = blockDim.x;
+  const OptTensor& t = a.t;
+  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const long long e0 = r * a.cols, end = e0 + a.cols;
+    const bool vec = t.vec && (int)threadIdx.x * 8 < a.cols;      // the last lanes of a row may have nothing
+    float p[8], g[8], m[8], v[8];
+    if (t.vec && !vec) {
+#pragma unroll
+      for (int j = 0; j < 8; j++) p[j] = g[j] = m[j] = v[j] = 0.0f;
+    } else {
+      if (MASTER)
+        opt_load<float>(t.master, e0, end, vec, threadIdx.x, lanes, p);
+      else
+        opt_load<P>(t.param, e0, end, vec, threadIdx.x, lanes, p);
+      opt_load<G>(t.grad, e0, end, vec, threadIdx.x, lanes, g);
+      opt_load<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m);
+      opt_load<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v);
+    }
+    float gp = 0.0f, pp = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      g[j] *= co.clip;
+      gp = fmaf(g[j], p[j], gp);
+      pp = fmaf(p[j], p[j], pp);
+    }
+    const float2 dots = cta_sum2(gp, pp, part[0], warps);
+    const float along = dots.y > 0.0f ? dots.x / dots.y : 0.0f;
+    float len = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      opt_moments(a.s, g[j] - along * p[j], m[j], v[j]);
+      p[j] = adamw_param(a.s, co, p[j], m[j], v[j]);
+      len = fmaf(p[j], p[j], len);
+    }
+    len = cta_sum2(len, 0.0f, part[1], warps).x;
+    const float scale = len > 0.0f ? 1.0f / sqrtf(len) : 1.0f;      // a row of zeros stays one
+#pragma unroll
+    for (int j = 0; j < 8; j++) p[j] *= scale;
+    if (t.vec && !vec) continue;
+    opt_store<P>(t.param, e0, end, vec, threadIdx.x, lanes, p);
+    if (MASTER) opt_store<float>(t.master, e0, end, vec, threadIdx.x, lanes, p);
+    opt_store<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m);
+    opt_store<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v);
+  }
+  opt_advance(a.s, co.t);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------
+static size_t opt_size(int dt) { return dt == FLEXSAE_F32 ? 4 : 2; }
+static bool opt_dtype(int dt) { return dt == FLEXSAE_F32 || dt == FLEXSAE_BF16 || dt == FLEXSAE_F16; }
+static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+
+constexpr int64_t kOptMaxTensors = 1 << 16;
+constexpr int64_t kOptMaxNumel = 1ll << 40;
+constexpr int kOptGrid = 148 * 8;       // CTAs of a launch at most; each takes every gridDim-th chunk
+constexpr int kSmallBatch = 16, kLargeBatch = 256;
+
+// A stretch of memory that a step reads or writes.
+struct Stretch {
+  uintptr_t begin, end;
+  bool written;
+};
+
+static int check_scalars(const int64_t* step, double lr, double beta1, double beta2, double eps, double weight_decay,
+                         const float* norm, double max_norm) {
+  if (!step) return fail(FLEXSAE_EINVAL, "null pointer argument: step");
+  if (!aligned(step, 8)) return fail(FLEXSAE_EINVAL, "step must be 8-byte aligned");
+  if (!(lr >= 0.0 && lr <= FLT_MAX)) return fail(FLEXSAE_EINVAL, "lr = %g is not a finite number >= 0", lr);
+  if (!(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0)) return fail(FLEXSAE_EINVAL, "betas %g, %g outside [0, 1)", beta1, beta2);
+  if (!(eps >= FLT_MIN && eps <= FLT_MAX)) return fail(FLEXSAE_EINVAL, "eps = %g must be a normal 32-bit number > 0", eps);
+  if (!(weight_decay >= 0.0 && weight_decay <= FLT_MAX)) return fail(FLEXSAE_EINVAL, "weight_decay = %g is not a finite number >= 0", weight_decay);
+  if (norm && !(max_norm > 0.0)) return fail(FLEXSAE_EINVAL, "max_norm = %g must be positive", max_norm);
+  return 0;
+}
+
+static OptScalars make_scalars(int64_t* step, double lr, const float* lr_device, double beta1, double beta2, double eps,
+                               double weight_decay, const float* norm, double max_norm, uint32_t seed) {
+  OptScalars s;
+  s.step = reinterpret_cast<unsigned long long*>(step);
+  s.norm = norm;
+  s.lr_device = lr_device;
+  s.lr = lr;
+  s.weight_decay = weight_decay;
+  s.log_beta1 = log(beta1);
+  s.log_beta2 = log(beta2);
+  s.beta1 = (float)beta1;
+  s.one_minus_beta1 = (float)(1.0 - beta1);
+  s.beta2 = (float)beta2;
+  s.one_minus_beta2 = (float)(1.0 - beta2);
+  s.eps = (float)eps;
+  s.max_norm = (float)max_norm;
+  s.seed = seed;
+  s.advance = 0;
+  return s;
+}
+
+// Checks one tensor's description and notes the memory that it reads and writes.
+static int check_tensor(const flexsae_optim_tensor& t, int64_t i, int state_bits, bool rows, Stretch* out, int* used) {
+  const long long at = (long long)i;
+  if (!opt_dtype(t.param_dtype)) return fail(FLEXSAE_EINVAL, "tensor %lld: unknown dtype code %d", at, t.param_dtype);
+  if (t.grad_dtype != t.param_dtype && t.grad_dtype != FLEXSAE_F32)
+    return fail(FLEXSAE_EINVAL, "tensor %lld: the gradient's type (code %d) must be the parameter's or fp32", at, t.grad_dtype);
+  if (t.master && t.param_dtype == FLEXSAE_F32) return fail(FLEXSAE_EINVAL, "tensor %lld: a master copy goes with 16-bit parameters only", at);
+  if (t.numel < 0 || t.numel > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^40]", at, (long long)t.numel);
+  *used = 0;
+  if (t.numel == 0) return 0;
+  if (rows) {
+    if (t.cols < 1 || t.numel % t.cols) return fail(FLEXSAE_EINVAL, "tensor %lld: %lld elements are not rows of %lld", at, (long long)t.numel, (long long)t.cols);
+    if (t.cols > kOptMaxRow) return fail(FLEXSAE_EUNSUPPORTED, "tensor %lld: rows of %lld elements, at most %d are supported", at, (long long)t.cols, kOptMaxRow);
+  }
+  if (!t.param || !t.grad || !t.exp_avg || !t.exp_avg_sq) return fail(FLEXSAE_EINVAL, "tensor %lld: null pointer argument", at);
+  const size_t n = (size_t)t.numel, ps = opt_size(t.param_dtype), gs = opt_size(t.grad_dtype), ss = state_bits == 8 ? 1 : 4;
+  const size_t scales = state_bits == 8 ? (n + kOptBlock - 1) / kOptBlock * 4 : 0;
+  if (state_bits == 8 && (!t.exp_avg_scale || !t.exp_avg_sq_scale)) return fail(FLEXSAE_EINVAL, "tensor %lld: null pointer argument: scales", at);
+  const struct { const void* p; size_t bytes, align; bool written; } use[] = {
+      {t.param, n * ps, ps, true}, {t.grad, n * gs, gs, false}, {t.exp_avg, n * ss, ss, true}, {t.exp_avg_sq, n * ss, ss, true},
+      {t.master, t.master ? n * 4 : 0, 4, true}, {t.exp_avg_scale, scales, 4, true}, {t.exp_avg_sq_scale, scales, 4, true}};
+  for (const auto& u : use) {
+    if (!u.bytes) continue;
+    if (!aligned(u.p, u.align)) return fail(FLEXSAE_EINVAL, "tensor %lld: a pointer is not aligned to its elements", at);
+    const uintptr_t b = reinterpret_cast<uintptr_t>(u.p);
+    out[(*used)++] = Stretch{b, b + u.bytes, u.written};
+  }
+  return 0;
+}
+
+// Tensors given twice, states that overlap: two CTAs would write the same memory.
+static int check_overlap(Stretch* s, int64_t n) {
+  std::sort(s, s + n, [](const Stretch& a, const Stretch& b) { return a.begin < b.begin; });
+  uintptr_t end = 0, end_written = 0;
+  for (int64_t i = 0; i < n; i++) {
+    if (s[i].begin < end_written || (s[i].written && s[i].begin < end))
+      return fail(FLEXSAE_EINVAL, "a tensor is given twice, or two of the tensors overlap in memory");
+    end = std::max(end, s[i].end);
+    if (s[i].written) end_written = std::max(end_written, s[i].end);
+  }
+  return 0;
+}
+
+static int check_tensors(const flexsae_optim_tensor* t, int64_t n, int state_bits, bool rows) {
+  if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
+  if (n == 0) return 0;
+  if (!t) return fail(FLEXSAE_EINVAL, "null pointer argument: tensors");
+  Stretch few[7 * kSmallBatch];
+  Stretch* all = n <= kSmallBatch ? few : new (std::nothrow) Stretch[7 * n];
+  if (!all) return fail(FLEXSAE_EINVAL, "out of host memory");
+  int64_t used = 0;
+  int rc = 0;
+  for (int64_t i = 0; i < n && rc == 0; i++) {
+    int k = 0;
+    rc = check_tensor(t[i], i, state_bits, rows, all + used, &k);
+    used += k;
+  }
+  if (rc == 0) rc = check_overlap(all, used);
+  if (all != few) delete[] all;
+  return rc;
+}
+
+static OptTensor make_tensor(const flexsae_optim_tensor& t, int64_t i, int state_bits) {
+  OptTensor d;
+  d.param = t.param;
+  d.grad = t.grad;
+  d.exp_avg = t.exp_avg;
+  d.exp_avg_sq = t.exp_avg_sq;
+  d.exp_avg_scale = t.exp_avg_scale;
+  d.exp_avg_sq_scale = t.exp_avg_sq_scale;
+  d.master = t.master;
+  d.numel = t.numel;
+  d.index = (int)i;
+  const size_t state_align = state_bits == 8 ? 8 : 16;
+  d.vec = aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.master, 16) && aligned(t.exp_avg, state_align) &&
+          aligned(t.exp_avg_sq, state_align);
+  return d;
+}
+
+// Kernels are compiled per (parameter type, gradient type, master copy): 0 fp32; then bf16 and fp16,
+// each with gradients of its own type or fp32, without and with a master copy.
+constexpr int kOptKinds = 9;
+static int kind_of(const flexsae_optim_tensor& t) {
+  if (t.param_dtype == FLEXSAE_F32) return 0;
+  return 1 + (t.param_dtype == FLEXSAE_F16 ? 4 : 0) + (t.grad_dtype == FLEXSAE_F32 ? 2 : 0) + (t.master ? 1 : 0);
+}
+
+#define FLEXSAE_OPT_KINDS(kind, CALL)                         \
+  switch (kind) {                                             \
+    case 0: CALL(float, float, false); break;                 \
+    case 1: CALL(__nv_bfloat16, __nv_bfloat16, false); break; \
+    case 2: CALL(__nv_bfloat16, __nv_bfloat16, true); break;  \
+    case 3: CALL(__nv_bfloat16, float, false); break;         \
+    case 4: CALL(__nv_bfloat16, float, true); break;          \
+    case 5: CALL(__half, __half, false); break;               \
+    case 6: CALL(__half, __half, true); break;                \
+    case 7: CALL(__half, float, false); break;                \
+    default: CALL(__half, float, true); break;                \
+  }
+
+template <int N>
+static cudaError_t launch_adamw(const OptBatch<N>& b, int kind, int state_bits, cudaStream_t st) {
+  const unsigned grid = std::max(1u, std::min(b.chunks, (unsigned)kOptGrid));
+#define CALL_ADAMW(P, G, M)                                                                       \
+  if (state_bits == 8) adamw8_kernel<P, G, M, N><<<grid, kOptThreads, 0, st>>>(b);                \
+  else adamw_kernel<P, G, M, N><<<grid, kOptThreads, 0, st>>>(b)
+  FLEXSAE_OPT_KINDS(kind, CALL_ADAMW)
+#undef CALL_ADAMW
+  t_launches++;
+  return cudaGetLastError();
+}
+
+// Launches the tensors ids[0..n) of one kind, at most N at a time.
+template <int N>
+static cudaError_t run_kind(const flexsae_optim_tensor* t, const int* ids, int n, int kind, int state_bits, const OptScalars& s,
+                            bool last_kind, cudaStream_t st) {
+  int k = 0;
+  do {
+    OptBatch<N> b;
+    b.s = s;
+    b.count = 0;
+    unsigned long long chunks = 0;
+    b.first[0] = 0;
+    while (k < n && b.count < N) {
+      const OptTensor d = make_tensor(t[ids[k]], ids[k], state_bits);
+      const unsigned long long c = ((unsigned long long)d.numel + kOptChunk - 1) / kOptChunk;
+      if (b.count && chunks + c > 0x7fffffffull) break;
+      chunks += c;
+      b.t[b.count++] = d;
+      b.first[b.count] = (unsigned)chunks;
+      k++;
+    }
+    b.chunks = (unsigned)chunks;
+    b.s.advance = last_kind && k == n;
+    if (cudaError_t e = launch_adamw<N>(b, kind, state_bits, st)) return e;
+  } while (k < n);
+  return cudaSuccess;
+}
+
+static int adamw_impl(const flexsae_optim_tensor* t, int64_t n, int state_bits, const OptScalars& s, cudaStream_t st) {
+  // positions of the non-empty tensors, kind by kind
+  int few[kSmallBatch];
+  int* ids = n <= kSmallBatch ? few : new (std::nothrow) int[n];
+  if (!ids) return fail(FLEXSAE_EINVAL, "out of host memory");
+  int begin[kOptKinds + 1], used = 0, last = 0;
+  for (int kind = 0; kind < kOptKinds; kind++) {
+    begin[kind] = used;
+    for (int64_t i = 0; i < n; i++)
+      if (t[i].numel > 0 && kind_of(t[i]) == kind) ids[used++] = (int)i;
+    if (used > begin[kind]) last = kind;
+  }
+  begin[kOptKinds] = used;
+  cudaError_t e = cudaSuccess;
+  for (int kind = 0; kind <= last && e == cudaSuccess; kind++) {
+    const int m = begin[kind + 1] - begin[kind];
+    if (m == 0 && !(kind == last && used == 0)) continue;      // nothing to update: one launch still counts the step
+    e = m <= kSmallBatch ? run_kind<kSmallBatch>(t, ids + begin[kind], m, kind, state_bits, s, kind == last, st)
+                         : run_kind<kLargeBatch>(t, ids + begin[kind], m, kind, state_bits, s, kind == last, st);
+  }
+  if (ids != few) delete[] ids;
+  if (e != cudaSuccess) return fail((int)e, "AdamW launch failed: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+static cudaError_t launch_rows(const RowArgs& a, int kind, cudaStream_t st) {
+  const int warps = (a.cols + kOptBlock - 1) / kOptBlock;
+  const int per_sm = std::max(1, std::min(32, 64 / warps));
+  const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(a.rows, 148ll * per_sm));
+#define CALL_ROWS(P, G, M) adamw_unit_rows_kernel<P, G, M><<<grid, warps * 32, 0, st>>>(a)
+  FLEXSAE_OPT_KINDS(kind, CALL_ROWS)
+#undef CALL_ROWS
+  t_launches++;
+  return cudaGetLastError();
+}
+
+template <int N>
+static cudaError_t launch_norm(const NormBatch<N>& b, unsigned grid, cudaStream_t st) {
+  grad_norm_kernel<N><<<grid, kOptThreads, 0, st>>>(b);
+  t_launches++;
+  return cudaGetLastError();
+}
+
+}  // namespace flexsae
+
+using namespace flexsae;
+
+extern "C" {
+
+size_t flexsae_grad_norm_workspace_bytes(int64_t n) {
+  if (n < 0 || n > kOptMaxTensors) {
+    fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
+    return 0;
+  }
+  return (size_t)((n + kLargeBatch - 1) / kLargeBatch + 1) * kNormGrid * sizeof(double);
+}
+
+int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int32_t* dtypes_host, int64_t n,
+                      float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
+  t_launches = 0;
+  if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
+  if (!norm_out || !workspace || (n > 0 && (!grads_host || !numel_host || !dtypes_host))) return fail(FLEXSAE_EINVAL, "null pointer argument");
+  if (!aligned(workspace, 8)) return fail(FLEXSAE_EINVAL, "workspace must be 8-byte aligned");
+  const size_t need = flexsae_grad_norm_workspace_bytes(n);
+  if (workspace_bytes < need) return fail(FLEXSAE_EWORKSPACE, "gradient norm workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  for (int64_t i = 0; i < n; i++) {
+    if (!opt_dtype(dtypes_host[i])) return fail(FLEXSAE_EINVAL, "tensor %lld: unknown dtype code %d", (long long)i, dtypes_host[i]);
+    if (numel_host[i] < 0 || numel_host[i] > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^40]", (long long)i, (long long)numel_host[i]);
+    if (numel_host[i] > 0 && !grads_host[i]) return fail(FLEXSAE_EINVAL, "tensor %lld: null pointer argument", (long long)i);
+    if (!aligned(grads_host[i], opt_size(dtypes_host[i]))) return fail(FLEXSAE_EINVAL, "tensor %lld: a pointer is not aligned to its elements", (long long)i);
+  }
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  double* partial = reinterpret_cast<double*>(workspace);
+  int parts = 0;
+  cudaError_t e = cudaSuccess;
+  int64_t i = 0;
+  const auto gather = [&](auto& b, int most) {      // the next tensors, as many as fit
+    unsigned long long chunks = 0;
+    b.count = 0;
+    b.first[0] = 0;
+    for (; i < n && b.count < most; i++) {
+      const unsigned long long c = ((unsigned long long)numel_host[i] + kNormChunk - 1) / kNormChunk;
+      if (c == 0) continue;
+      if (b.count && chunks + c > 0x7fffffffull) break;
+      chunks += c;
+      b.grad[b.count] = grads_host[i];
+      b.numel[b.count] = numel_host[i];
+      b.dtype[b.count] = (unsigned char)dtypes_host[i];
+      b.vec[b.count] = aligned(grads_host[i], 16);
+      b.first[++b.count] = (unsigned)chunks;
+    }
+    b.chunks = (unsigned)chunks;
+    b.partial = partial + parts;
+    if (!b.count) return;
+    const unsigned grid = std::min(b.chunks, (unsigned)kNormGrid);
+    e = launch_norm(b, grid, st);
+    parts += (int)grid;
+  };
+  while (i < n && e == cudaSuccess) {
+    if (n <= kSmallBatch) {
+      NormBatch<kSmallBatch> b;
+      gather(b, kSmallBatch);
+    } else {
+      NormBatch<kLargeBatch> b;
+      gather(b, kLargeBatch);
+    }
+  }
+  if (e == cudaSuccess) {
+    grad_norm_finish_kernel<<<1, kOptThreads, 0, st>>>(partial, parts, norm_out);
+    t_launches++;
+    e = cudaGetLastError();
+  }
+  if (e != cudaSuccess) return fail((int)e, "gradient norm launch failed: %s", cudaGetErrorString(e));
+  return 0;
+}
+
+int flexsae_adamw_step(const flexsae_optim_tensor* tensors_host, int64_t n, int state_bits, int64_t* step, double lr,
+                       const float* lr_device, double beta1, double beta2, double eps, double weight_decay, const float* norm,
+                       double max_norm, uint32_t seed, void* stream) {
+  t_launches = 0;
+  if (state_bits != 32 && state_bits != 8) return fail(FLEXSAE_EINVAL, "states of %d bits: 32 and 8 are supported", state_bits);
+  if (int rc = check_scalars(step, lr, beta1, beta2, eps, weight_decay, norm, max_norm)) return rc;
+  if (int rc = check_tensors(tensors_host, n, state_bits, false)) return rc;
+  return adamw_impl(tensors_host, n, state_bits,
+                    make_scalars(step, lr, lr_device, beta1, beta2, eps, weight_decay, norm, max_norm, seed),
+                    reinterpret_cast<cudaStream_t>(stream));
+}
+
+int flexsae_adamw_unit_rows_step(const flexsae_optim_tensor* tensors_host, int64_t n, int64_t* step, double lr,
+                                 const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                                 const float* norm, double max_norm, void* stream) {
+  t_launches = 0;
+  if (int rc = check_scalars(step, lr, beta1, beta2, eps, weight_decay, norm, max_norm)) return rc;
+  if (int rc = check_tensors(tensors_host, n, 32, true)) return rc;
+  const OptScalars s = make_scalars(step, lr, lr_device, beta1, beta2, eps, weight_decay, norm, max_norm, 0);
+  cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+  int64_t last = -1;
+  for (int64_t i = 0; i < n; i++)
+    if (tensors_host[i].numel > 0) last = i;
+  if (last < 0) return adamw_impl(nullptr, 0, 32, s, st);        // nothing to update: the step still counts
+  for (int64_t i = 0; i <= last; i++) {
+    const flexsae_optim_tensor& t = tensors_host[i];
+    if (t.numel == 0) continue;
+    RowArgs a;
+    a.s = s;
+    a.s.advance = i == last;
+    a.t = make_tensor(t, i, 32);
+    a.t.vec = a.t.vec && t.cols % 8 == 0;
+    a.rows = t.numel / t.cols;
+    a.cols = (int)t.cols;
+    if (cudaError_t e = launch_rows(a, kind_of(t), st)) return fail((int)e, "unit-row AdamW launch failed: %s", cudaGetErrorString(e));
+  }
+  return 0;
+}
+
+}  // extern "C"

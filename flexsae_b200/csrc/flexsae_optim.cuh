@@ -1,0 +1,178 @@
+// Argument blocks and device helpers of the optimizer kernels (gradient norm, AdamW steps).
+//
+// All of them stream their tensors once, so the unit of work is the same everywhere: one warp takes
+// 256 consecutive elements, eight per lane.  Lane l holds elements 8 l .. 8 l + 7 where every tensor
+// involved is 16-byte aligned and the 256 elements are all there (16-byte loads and stores), and
+// elements l, 32 + l, 64 + l, ... otherwise (the lanes of a warp then still touch consecutive memory).
+#pragma once
+
+#include <cuda_fp8.h>
+#include <float.h>
+
+#include "flexsae_common.cuh"
+#include "flexsae_host.cuh"
+
+namespace flexsae {
+
+constexpr int kOptThreads = 256;
+constexpr int kOptBlock = 256;                              // elements of a warp's unit = elements that share one scale
+constexpr int kOptChunk = kOptThreads / 32 * kOptBlock;     // elements of a CTA's unit
+constexpr int kOptMaxRow = 8192;                            // longest row of the unit-row step
+
+// Tensor lists travel as kernel arguments (up to 32764 bytes), so a call needs no copy to the device
+// and a captured graph holds its own list.
+struct OptTensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  float* master;
+  long long numel;
+  int index;     // position in the caller's list (part of the random key)
+  int vec;       // every pointer allows 16-byte (8-bit states: 8-byte) accesses
+};
+
+struct OptScalars {
+  unsigned long long* step;   // steps taken (low 40 bits) and, while a step runs, finished CTAs (high 24 bits)
+  const float* norm;          // gradient norm, or NULL
+  const float* lr_device;     // learning rate on the device, or NULL
+  double lr, weight_decay, log_beta1, log_beta2;
+  float beta1, one_minus_beta1, beta2, one_minus_beta2, eps, max_norm;
+  unsigned seed;
+  int advance;                // this launch is the last of its step
+};
+
+template <int N>
+struct OptBatch {
+  OptScalars s;
+  unsigned chunks;
+  int count;
+  unsigned first[N + 1];      // first chunk of each tensor
+  OptTensor t[N];
+};
+
+struct OptCoefs {
+  float clip;     // factor of the gradients
+  float decay;    // 1 - lr * weight_decay
+  float rate;     // lr / (1 - beta1^t)
+  float root;     // 1 / sqrt(1 - beta2^t)
+  unsigned long long t;
+};
+
+constexpr unsigned long long kStepMask = (1ull << 40) - 1;
+
+// The numbers that are the same for every element of a step.  False: the gradient norm is not finite
+// and the step does not take place.
+__device__ __forceinline__ bool opt_coefs(const OptScalars& s, OptCoefs& c) {
+  c.clip = 1.0f;
+  if (s.norm) {
+    const float n = *s.norm;
+    if (!(fabsf(n) <= FLT_MAX)) return false;
+    c.clip = fminf(__fmul_rn(__frcp_rn(__fadd_rn(n, 1e-6f)), s.max_norm), 1.0f);
+  }
+  c.t = (*reinterpret_cast<volatile unsigned long long*>(s.step) & kStepMask) + 1;
+  const double lr = s.lr_device ? (double)*s.lr_device : s.lr;
+  const double t = (double)c.t;
+  c.decay = (float)(1.0 - lr * s.weight_decay);
+  c.rate = __fdiv_rn((float)lr, -expm1f((float)(t * s.log_beta1)));   // 1 - b^t without cancellation
+  c.root = __frcp_rn(__fsqrt_rn(-expm1f((float)(t * s.log_beta2))));
+  return true;
+}
+
+// Every CTA reads the step count when it starts; the last CTA to finish writes the next one, so no CTA
+// can see it and no other launch is needed.
+__device__ __forceinline__ void opt_advance(const OptScalars& s, unsigned long long t) {
+  if (!s.advance) return;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    const unsigned long long before = atomicAdd(s.step, kStepMask + 1);
+    if ((before >> 40) == gridDim.x - 1) *reinterpret_cast<volatile unsigned long long*>(s.step) = t;
+  }
+}
+
+// Tensor that owns chunk c, searched upwards from tensor i.
+template <int N>
+__device__ __forceinline__ int opt_find(const OptBatch<N>& b, unsigned c, int i) {
+  if (c < b.first[i + 1]) return i;
+  int lo = i + 1, hi = b.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (c < b.first[mid + 1]) hi = mid; else lo = mid + 1;
+  }
+  return lo;
+}
+
+// ---- eight elements of a lane ---------------------------------------------------------------------
+template <typename T>
+__device__ __forceinline__ float opt_widen(T x) { return x; }
+template <>
+__device__ __forceinline__ float opt_widen<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float opt_widen<__half>(__half x) { return __half2float(x); }
+template <typename T>
+__device__ __forceinline__ T opt_narrow(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 opt_narrow<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half opt_narrow<__half>(float x) { return __float2half_rn(x); }
+
+// `e0` is the first element of the unit, `lane` / `lanes` this thread's place in the team that shares it.
+template <typename T>
+__device__ __forceinline__ void opt_load(const void* base, long long e0, long long end, bool vec, int lane, int lanes, float* out) {
+  if (vec) {
+    constexpr int V = Pack<T>::VEC;
+    const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(base) + e0 + lane * 8);
+#pragma unroll
+    for (int i = 0; i < 8 / V; i++) Pack<T>::unpack(q[i], out + i * V);
+  } else {
+    const T* q = reinterpret_cast<const T*>(base);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const long long e = e0 + j * lanes + lane;
+      out[j] = e < end ? opt_widen<T>(q[e]) : 0.0f;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void opt_store(void* base, long long e0, long long end, bool vec, int lane, int lanes, const float* in) {
+  if (vec) {
+    constexpr int V = Pack<T>::VEC;
+    uint4* q = reinterpret_cast<uint4*>(reinterpret_cast<T*>(base) + e0 + lane * 8);
+#pragma unroll
+    for (int i = 0; i < 8 / V; i++) q[i] = Pack<T>::pack(in + i * V);
+  } else {
+    T* q = reinterpret_cast<T*>(base);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const long long e = e0 + j * lanes + lane;
+      if (e < end) q[e] = opt_narrow<T>(in[j]);
+    }
+  }
+}
+
+// The two running averages.  Multiplications and additions are rounded one by one (no fused
+// multiply-add), so that the states -- and with them the 8-bit codes -- are the same bits wherever the
+// formula is written out in 32-bit arithmetic.
+__device__ __forceinline__ void opt_moments(const OptScalars& s, float g, float& m, float& v) {
+  m = __fadd_rn(__fmul_rn(s.beta1, m), __fmul_rn(s.one_minus_beta1, g));
+  v = __fadd_rn(__fmul_rn(s.beta2, v), __fmul_rn(s.one_minus_beta2, __fmul_rn(g, g)));
+}
+
+// ---- 8-bit states -----------------------------------------------------------------------------------
+// A 32-bit integer mixing function: two multiplications between three xor-shifts.
+__device__ __forceinline__ unsigned opt_mix(unsigned x) {
+  x = (x ^ (x >> 16)) * 0x7feb352du;
+  x = (x ^ (x >> 15)) * 0x846ca68bu;
+  return x ^ (x >> 16);
+}
+
+// Key of one tensor in one step; the 32 random bits of elements 2 j and 2 j + 1 are
+// mix(low 32 bits of j ^ (key + high bits of j)).
+__device__ __forceinline__ unsigned opt_key(unsigned seed, unsigned long long t, int index) {
+  return opt_mix(opt_mix(opt_mix((unsigned)t) + (unsigned)index) + seed);
+}
+
+}  // namespace flexsae

@@ -1,0 +1,395 @@
+"""The optimizer step behind the decoder losses: gradient norm, AdamW with 32-bit or 8-bit states,
+AdamW on a decoder whose rows are kept at unit length.
+
+The reference ends at the gradients (torch-ext/flex_sae/hierarchical_kernels.py:288-299); its callers
+take the step with the optimizer of their choice.  Here one launch updates all tensors of a model:
+
+    opt = flexsae_b200.optim.AdamW([{"params": [w_enc, b_enc, b_dec]},
+                                    {"params": [w_dec], "unit_rows": True}], lr=1e-4, max_norm=1.0)
+    loss.backward()
+    opt.step()
+    opt.zero_grad()
+
+``AdamW`` is a ``torch.optim.Optimizer`` over four functions that can be called on their own:
+``grad_norm``, ``adamw_step``, ``adamw8_step``, ``adamw_unit_rows_step``.  They work in place on lists of
+tensors, on the current stream, without a synchronisation; a step's number, its clipping factor and
+whether it takes place at all (it does not when the gradient norm is not finite) are decided on the
+device, so a step can be captured in a CUDA graph and replayed.  Results are the same bits every time,
+so replicas that step on the same gradients stay equal.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import _native as nv
+from . import losses as _losses
+
+#: elements that share one scale of the 8-bit states
+BLOCK = 256
+#: types of the 8-bit states: first moment, second moment
+STATE8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
+
+_WORDS = 10          # 64-bit words of flexsae_optim_tensor
+_Tensors = Sequence[torch.Tensor]
+_Masters = Sequence[Optional[torch.Tensor]]
+
+
+def state8_blocks(numel: int) -> int:
+    """Number of scales that go with ``numel`` 8-bit values."""
+    return -(-numel // BLOCK)
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """True if the elements fill a stretch of memory without gaps, each once (in any order of dimensions)."""
+    if t.is_contiguous():
+        return True
+    expected = 1
+    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != expected:
+            return t.numel() == 0
+        expected *= size
+    return True
+
+
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return all(n == 1 or x == y for x, y, n in zip(a.stride(), b.stride(), a.shape))
+
+
+def _check_word(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> int:
+    if not isinstance(t, torch.Tensor) or t.numel() != 1:
+        raise ValueError(f"{name} must be a tensor of one element")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device != dev:
+        raise RuntimeError(f"{name} is on {t.device}, the parameters are on {dev}")
+    return t.data_ptr()
+
+
+def _check_list(name: str, ts: Optional[_Tensors], params: _Tensors, dtype: torch.dtype, dev: torch.device) -> None:
+    if len(ts) != len(params):
+        raise ValueError(f"{len(ts)} tensors in {name}, {len(params)} parameters")
+    for t, p in zip(ts, params):
+        if t.dtype != dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.device != dev:
+            raise RuntimeError(f"a tensor in {name} is on {t.device}, the parameters are on {dev}")
+        if t.shape != p.shape or not _same_layout(t, p):
+            raise ValueError(f"a tensor in {name} has shape {tuple(t.shape)} and strides {t.stride()}, "
+                             f"its parameter {tuple(p.shape)} and {p.stride()}")
+
+
+def _check_scales(name: str, ts: _Tensors, params: _Tensors, dev: torch.device) -> None:
+    if len(ts) != len(params):
+        raise ValueError(f"{len(ts)} tensors in {name}, {len(params)} parameters")
+    for t, p in zip(ts, params):
+        if t.dtype != torch.float32:
+            raise TypeError(f"{name} must be float32, got {t.dtype}")
+        if t.device != dev:
+            raise RuntimeError(f"a tensor in {name} is on {t.device}, the parameters are on {dev}")
+        if t.shape != (state8_blocks(p.numel()),) or not t.is_contiguous():
+            raise ValueError(f"{name} of {p.numel()} elements is contiguous float32 [{state8_blocks(p.numel())}], "
+                             f"got {tuple(t.shape)}")
+
+
+def _check_params(params: _Tensors, grads: _Tensors, rows: bool) -> Tuple[torch.device, List[torch.Tensor]]:
+    """Checks parameters and gradients; returns the device and the gradients in their parameters' layout."""
+    if len(grads) != len(params):
+        raise ValueError(f"{len(grads)} gradients, {len(params)} parameters")
+    dev, got = params[0].device, []
+    if dev.type != "cuda":
+        raise RuntimeError("flexsae_b200.optim needs CUDA tensors: there is no CPU path")
+    for p, g in zip(params, grads):
+        if p.dtype not in nv.DTYPE_CODES:
+            raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
+        if g.layout != torch.strided:
+            raise TypeError(f"gradients must be dense tensors, got {g.layout}")
+        if g.dtype != p.dtype and g.dtype != torch.float32:
+            raise TypeError(f"the gradient of a {p.dtype} parameter must have its type or float32, got {g.dtype}")
+        if p.device != dev or g.device != dev:
+            raise RuntimeError(f"parameters and gradients must be on one device, got {p.device} and {g.device} beside {dev}")
+        if g.shape != p.shape:
+            raise ValueError(f"a gradient has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
+        if not _dense(p):
+            raise ValueError(f"a parameter of shape {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
+        if rows and (p.dim() != 2 or not p.is_contiguous()):
+            raise ValueError(f"unit rows need a contiguous [F, D] parameter, got {tuple(p.shape)} with strides {p.stride()}")
+        if not _same_layout(g, p):
+            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
+        got.append(g)
+    return dev, got
+
+
+def _step(entry: str, params: _Tensors, grads: _Tensors, states: Sequence[Optional[_Tensors]], step: torch.Tensor, lr, betas, eps,
+          weight_decay, masters, norm, max_norm, rows: bool = False, bits: int = 32, seed: int = 0) -> None:
+    lib = nv.load()
+    params = [p.detach() for p in params]
+    if not params:
+        raise ValueError("no parameters")
+    dev, grads = _check_params(params, grads, rows)
+    exp_avgs, scales, exp_avg_sqs, sq_scales = states
+    kinds = STATE8_DTYPES if bits == 8 else (torch.float32, torch.float32)
+    _check_list("exp_avgs", exp_avgs, params, kinds[0], dev)
+    _check_list("exp_avg_sqs", exp_avg_sqs, params, kinds[1], dev)
+    if bits == 8:
+        _check_scales("exp_avg_scales", scales, params, dev)
+        _check_scales("exp_avg_sq_scales", sq_scales, params, dev)
+    if masters is not None:
+        if len(masters) != len(params):
+            raise ValueError(f"{len(masters)} masters, {len(params)} parameters")
+        held = [(t, p) for t, p in zip(masters, params) if t is not None]
+        if any(p.dtype == torch.float32 for _, p in held):
+            raise ValueError("masters go with 16-bit parameters only")
+        _check_list("masters", [t for t, _ in held], [p for _, p in held], torch.float32, dev)
+    step_ptr = _check_word("step", step, torch.int64, dev)
+    lr_ptr = None
+    if isinstance(lr, torch.Tensor):
+        lr, lr_ptr = 0.0, _check_word("lr", lr, torch.float32, dev)
+    if not (math.isfinite(lr) and lr >= 0):
+        raise ValueError(f"lr must be a finite number >= 0, got {lr}")
+    if not all(0 <= b < 1 for b in betas):
+        raise ValueError(f"betas must be in [0, 1), got {betas}")
+    if not (math.isfinite(eps) and eps >= 2.0 ** -126):
+        raise ValueError(f"eps must be a normal float32 number > 0, got {eps}")
+    if not (math.isfinite(weight_decay) and weight_decay >= 0):
+        raise ValueError(f"weight_decay must be a finite number >= 0, got {weight_decay}")
+    if max_norm is not None and (norm is None or not max_norm > 0):
+        raise ValueError("max_norm must be positive and goes with norm")
+    norm_ptr = None if norm is None else _check_word("norm", norm, torch.float32, dev)
+    if not 0 <= seed < 2 ** 32:
+        raise ValueError(f"seed must be in [0, 2**32), got {seed}")
+    n = len(params)
+    zeros = [0] * n
+    columns = (
+        [p.data_ptr() for p in params], [g.data_ptr() for g in grads],
+        [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
+        [t.data_ptr() for t in scales] if bits == 8 else zeros, [t.data_ptr() for t in sq_scales] if bits == 8 else zeros,
+        [0 if t is None else t.data_ptr() for t in masters] if masters is not None else zeros,
+        [p.numel() for p in params], [p.shape[-1] for p in params] if rows else zeros,
+        [nv.DTYPE_CODES[p.dtype] | nv.DTYPE_CODES[g.dtype] << 32 for p, g in zip(params, grads)])
+    table = (ctypes.c_int64 * (_WORDS * n))()
+    for k, column in enumerate(columns):
+        table[k::_WORDS] = column
+    tail = [step_ptr, float(lr), lr_ptr, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), norm_ptr,
+            math.inf if max_norm is None else float(max_norm)]
+    with torch.cuda.device(dev):
+        stream = torch.cuda.current_stream(dev).cuda_stream
+        if rows:
+            rc = lib.flexsae_adamw_unit_rows_step(table, n, *tail, stream)
+        else:
+            rc = lib.flexsae_adamw_step(table, n, bits, *tail, seed, stream)
+    nv.check(rc, entry)
+    _losses.launch_count += lib.flexsae_last_launch_count()
+    written = [*params, *exp_avgs, *exp_avg_sqs, *(t for t in masters or () if t is not None)]
+    torch.autograd.graph.increment_version(written)      # what autograd saved of them is out of date now
+
+
+def grad_norm(grads: _Tensors) -> torch.Tensor:
+    """``sqrt(sum of squares)`` over all tensors of a list (float32, bfloat16 or float16, mixed) as a
+    0-dim float32 tensor: the ``norm`` of the step functions.  The squares are added in 64 bits in a
+    fixed order: the result is reproducible, and finite whenever float32 can hold it."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("no gradients")
+    dev = grads[0].device
+    if dev.type != "cuda":
+        raise RuntimeError("flexsae_b200.optim needs CUDA tensors: there is no CPU path")
+    for i, g in enumerate(grads):
+        if g.layout != torch.strided:
+            raise TypeError(f"gradients must be dense tensors, got {g.layout}")
+        if g.dtype not in nv.DTYPE_CODES:
+            raise TypeError(f"gradients must be float32, bfloat16 or float16, got {g.dtype}")
+        if g.device != dev:
+            raise RuntimeError(f"gradients must be on one device, got {g.device} beside {dev}")
+        if not _dense(g):
+            grads[i] = g.contiguous()
+    lib = nv.load()
+    n = len(grads)
+    with torch.cuda.device(dev):
+        norm = torch.empty((), dtype=torch.float32, device=dev)
+        ws = torch.empty(lib.flexsae_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
+        rc = lib.flexsae_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
+                                   (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
+                                   (ctypes.c_int32 * n)(*[nv.DTYPE_CODES[g.dtype] for g in grads]), n, norm.data_ptr(),
+                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
+    nv.check(rc, "flexsae_grad_norm")
+    _losses.launch_count += lib.flexsae_last_launch_count()
+    return norm
+
+
+def adamw_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sqs: _Tensors, step: torch.Tensor, *,
+               lr: Union[float, torch.Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 0.01, masters: Optional[_Masters] = None, norm: Optional[torch.Tensor] = None,
+               max_norm: Optional[float] = None) -> None:
+    """One AdamW step over lists of tensors, in place:
+
+        g = c grad                       m = b1 m + (1 - b1) g          v = b2 v + (1 - b2) g^2
+        p = p (1 - lr weight_decay) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+
+    ``params`` (float32, bfloat16 or float16, mixed), ``grads`` of the same types or float32, float32
+    states in their parameters' layout.  ``step``: int64 on the device, steps taken so far; t is one
+    more, and the call leaves t there.  ``masters``: float32 copies of 16-bit parameters that hold the
+    exact values (None where a parameter has none); the parameters are their roundings.  ``lr``: a number, or a float32 tensor on the
+    device (which a captured graph follows).  ``norm``: the norm of all gradients, from ``grad_norm``;
+    with it c = min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves everything as it
+    was.  A tensor given twice, or tensors that overlap, are refused."""
+    _step("flexsae_adamw_step", params, grads, (exp_avgs, None, exp_avg_sqs, None), step, lr, betas, eps, weight_decay, masters,
+          norm, max_norm)
+
+
+def adamw8_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_scales: _Tensors, exp_avg_sqs: _Tensors,
+                exp_avg_sq_scales: _Tensors, step: torch.Tensor, *, lr: Union[float, torch.Tensor],
+                betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.01,
+                masters: Optional[_Masters] = None, norm: Optional[torch.Tensor] = None, max_norm: Optional[float] = None,
+                seed: int = 0) -> None:
+    """``adamw_step`` with states of 8 bits: ``exp_avgs`` float8_e4m3fn and ``exp_avg_sqs`` float8_e5m2 in
+    their parameters' layout, each with one float32 scale for every ``BLOCK`` elements in memory order
+    (``state8_blocks(numel)`` of them; the value is code * scale).  The parameter is computed from the
+    new moments before they are rounded; then each goes at random to one of its two neighbours, so that
+    the rounding is right on average (rounding to nearest would never move a second moment, which a
+    step changes by a thousandth).  The random bits are a function of (seed, t, position in the list,
+    element).  A second moment is stored as at least 2^-16 of its scale.  An infinity or a NaN
+    stays with its own element."""
+    _step("flexsae_adamw_step", params, grads, (exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales), step, lr, betas, eps,
+          weight_decay, masters, norm, max_norm, bits=8, seed=seed)
+
+
+def adamw_unit_rows_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sqs: _Tensors, step: torch.Tensor, *,
+                         lr: Union[float, torch.Tensor], betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
+                         weight_decay: float = 0.01, masters: Optional[_Masters] = None, norm: Optional[torch.Tensor] = None,
+                         max_norm: Optional[float] = None) -> None:
+    """``adamw_step`` for decoders [F, D] (contiguous, D up to 8192) whose rows are kept at unit length: the
+    gradient's component along its row is taken out first (g -= (g.w / w.w) w), and after the step
+    the row is divided by its length.  A row of zeros stays one."""
+    _step("flexsae_adamw_unit_rows_step", params, grads, (exp_avgs, None, exp_avg_sqs, None), step, lr, betas, eps, weight_decay,
+          masters, norm, max_norm, rows=True)
+
+
+class AdamW(torch.optim.Optimizer):
+    """AdamW over the functions above, as a ``torch.optim.Optimizer``.
+
+    Per parameter group, beside ``lr`` (a number or a float32 tensor on the device), ``betas``, ``eps`` and
+    ``weight_decay``: ``state_bits`` (32 or 8), ``master_weights`` (float32 copies of 16-bit parameters in
+    the state), ``unit_rows`` (parameters [F, D] kept at unit rows; 32-bit states only) and ``seed`` (8-bit
+    states).  ``max_norm`` clips the norm over the gradients of all groups; ``skip_nonfinite`` measures
+    that norm without clipping.  With either, a step whose norm is not finite does not take place, and
+    ``norm`` holds the norm of the last step (a 0-dim tensor on the device).
+
+    A parameter without a gradient is passed over; its own step count does not move.  All parameters
+    live on one device."""
+
+    def __init__(self, params: Iterable, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
+                 eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32, master_weights: bool = False,
+                 unit_rows: bool = False, seed: int = 0, max_norm: Optional[float] = None, skip_nonfinite: bool = False):
+        if max_norm is not None and not max_norm > 0:
+            raise ValueError(f"max_norm must be positive, got {max_norm}")
+        self.max_norm, self.skip_nonfinite = max_norm, skip_nonfinite
+        self.norm: Optional[torch.Tensor] = None
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits,
+                                      master_weights=master_weights, unit_rows=unit_rows, seed=seed))
+
+    def add_param_group(self, param_group: dict) -> None:
+        super().add_param_group(param_group)
+        group = self.param_groups[-1]
+        try:
+            if group["state_bits"] not in (8, 32):
+                raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+            if group["unit_rows"] and group["state_bits"] != 32:
+                raise ValueError("unit_rows goes with 32-bit states")
+            for p in group["params"]:
+                if p.dtype not in nv.DTYPE_CODES:
+                    raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
+                if group["unit_rows"] and p.dim() != 2:
+                    raise ValueError(f"unit rows need [F, D] parameters, got {tuple(p.shape)}")
+        except (ValueError, TypeError):
+            self.param_groups.pop()
+            raise
+
+    def _new_state(self, p: torch.Tensor, group: dict, step: torch.Tensor) -> Dict[str, torch.Tensor]:
+        kinds = STATE8_DTYPES if group["state_bits"] == 8 else (torch.float32, torch.float32)
+        state = {"step": step, "exp_avg": torch.zeros_like(p, dtype=kinds[0], memory_format=torch.preserve_format),
+                 "exp_avg_sq": torch.zeros_like(p, dtype=kinds[1], memory_format=torch.preserve_format)}
+        if group["state_bits"] == 8:
+            for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                state[name] = torch.zeros(state8_blocks(p.numel()), dtype=torch.float32, device=p.device)
+        if group["master_weights"] and p.dtype != torch.float32:
+            state["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
+        return state
+
+    def _cohorts(self, group: dict) -> List[List[torch.Tensor]]:
+        """The group's parameters with gradients, those that share a step count together."""
+        active = [p for p in group["params"] if p.grad is not None]
+        new = [p for p in active if not self.state[p]]
+        if new:
+            step = torch.zeros((), dtype=torch.int64, device=new[0].device)
+            for p in new:
+                self.state[p].update(self._new_state(p, group, step))
+        if len(active) < len(group["params"]):      # who sits a step out keeps a count of its own
+            moving = {id(self.state[p]["step"]) for p in active}
+            for p in group["params"]:
+                if p.grad is None and self.state.get(p) and id(self.state[p]["step"]) in moving:
+                    self.state[p]["step"] = self.state[p]["step"].clone()
+        counts: Dict[int, List[torch.Tensor]] = {}
+        for p in active:
+            counts.setdefault(id(self.state[p]["step"]), []).append(p)
+        return list(counts.values())
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        self.norm = None
+        if self.max_norm is not None or self.skip_nonfinite:
+            grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
+            if grads:
+                self.norm = grad_norm(grads)
+        for group in self.param_groups:
+            for ps in self._cohorts(group):
+                self._step_cohort(group, ps)
+        return loss
+
+    def _step_cohort(self, group: dict, ps: List[torch.Tensor]) -> None:
+        states = [self.state[p] for p in ps]
+
+        def column(name: str) -> List[Optional[torch.Tensor]]:
+            return [s.get(name) for s in states]
+
+        grads, masters = [p.grad for p in ps], column("master")
+        kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
+                  masters=masters if any(t is not None for t in masters) else None, norm=self.norm, max_norm=self.max_norm)
+        if group["state_bits"] == 8:
+            adamw8_step(ps, grads, column("exp_avg"), column("exp_avg_scale"), column("exp_avg_sq"), column("exp_avg_sq_scale"),
+                        states[0]["step"], seed=group["seed"], **kw)
+        else:
+            step = adamw_unit_rows_step if group["unit_rows"] else adamw_step
+            step(ps, grads, column("exp_avg"), column("exp_avg_sq"), states[0]["step"], **kw)
+
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite, "norm": None}
+
+    def load_state_dict(self, state_dict: dict) -> None:
+        """Restores a ``state_dict``: the states keep their own types (the base class would turn them into the
+        parameters'), and parameters of a group that stand at the same step share their count again."""
+        super().load_state_dict(state_dict)
+        saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
+        params = [p for group in self.param_groups for p in group["params"]]
+        for i, p in zip(saved_ids, params):
+            for name, value in state_dict["state"].get(i, {}).items():
+                if name == "step":
+                    self.state[p][name] = torch.as_tensor(value).to(device=p.device, dtype=torch.int64).clone()
+                elif name.endswith("_scale"):
+                    self.state[p][name] = value.to(p.device).clone()
+                else:
+                    kept = torch.empty_like(p, dtype=value.dtype, memory_format=torch.preserve_format)
+                    self.state[p][name] = kept.copy_(value)
+        for group in self.param_groups:
+            counts: Dict[int, torch.Tensor] = {}
+            for p in group["params"]:
+                if self.state.get(p):
+                    step = self.state[p]["step"]
+                    self.state[p]["step"] = counts.setdefault(int(step), step)

@@ -301,6 +301,68 @@ int flexsae_loss_fwd_static_scratch(int kind, const int64_t* indices, const void
                                     int vals_dtype, int bias_dtype, int target_dtype,
                                     double inv_norm, int32_t* status, void* stream);
 
+/*
+ * The optimizer step behind the losses.  The reference has no counterpart: it stops at the gradients
+ * (torch-ext/flex_sae/hierarchical_kernels.py:288-299) and leaves the step to its caller.
+ *
+ * A step takes a host array of tensors.  All pointers in it are device pointers, aligned to their
+ * elements; 16-byte alignment (8 for 8-bit states) is faster.  Elements are taken in memory order, so
+ * the tensors of one entry have the same layout.  An entry with numel 0 is passed over.  Memory that
+ * a step writes must not overlap anything else in its list: this is checked, and refused.
+ */
+typedef struct flexsae_optim_tensor {
+  void* param;               /* updated in place */
+  const void* grad;
+  void* exp_avg;             /* first moment: float32, or e4m3 with 8-bit states */
+  void* exp_avg_sq;          /* second moment: float32, or e5m2 with 8-bit states */
+  float* exp_avg_scale;      /* 8-bit states: one float32 for every 256 elements (the last ones may be fewer) */
+  float* exp_avg_sq_scale;
+  float* master;             /* float32 copy of a 16-bit parameter that holds its exact value, or NULL */
+  int64_t numel;
+  int64_t cols;              /* length of a row (flexsae_adamw_unit_rows_step) */
+  int32_t param_dtype;
+  int32_t grad_dtype;        /* the parameter's, or FLEXSAE_F32 */
+} flexsae_optim_tensor;
+
+/*
+ * norm_out[0] = sqrt(sum of squares over all n gradients), float32.  Squares are added in 64 bits in a
+ * fixed order, so the result is the same bits every time and finite whenever it fits.  grads_host,
+ * numel_host and dtypes_host are host arrays of n entries; an empty list has norm 0.
+ */
+size_t flexsae_grad_norm_workspace_bytes(int64_t n);
+int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int32_t* dtypes_host, int64_t n,
+                      float* norm_out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One AdamW step over n tensors (decoupled weight decay), one launch for every combination of
+ * parameter type, gradient type and master copy in the list (up to 256 tensors each):
+ *   g = c grad                       m = beta1 m + (1 - beta1) g        v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ *   state_bits 32, or 8: m as e4m3 and v as e5m2 (see flexsae_optim_tensor), each block's scale its
+ *              largest absolute value / 448 or / 57344 (times 1 + 2^-20), the new values rounded at
+ *              random to one of their two neighbours so that the rounding is right on average.  The
+ *              random bits are a function of (seed, t, position in the list, element).  v is at least
+ *              2^-16 of its scale.  An infinity or NaN stays with its own element.
+ *   step       device int64: steps taken so far; t = step + 1, and the call leaves t there.  Calls that
+ *              share a step word must be ordered.
+ *   lr_device  optional device float32 that is used instead of lr (a captured graph follows it)
+ *   norm       optional device float32, the norm of all gradients: c = min(1, max_norm / (norm + 1e-6)),
+ *              and a norm that is not finite leaves everything as it was, the step word too.  NULL: c = 1.
+ */
+int flexsae_adamw_step(const flexsae_optim_tensor* tensors_host, int64_t n, int state_bits, int64_t* step, double lr,
+                       const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                       const float* norm, double max_norm, uint32_t seed, void* stream);
+
+/*
+ * The same step (32-bit states) for decoders [numel / cols, cols] whose rows are kept at unit length, in
+ * one pass: first the gradient's component along its row is taken out, g -= (g.w / w.w) w, and after
+ * the step the row is divided by its length.  A row of zeros stays one.  One launch for every tensor;
+ * rows of up to 8192 elements.
+ */
+int flexsae_adamw_unit_rows_step(const flexsae_optim_tensor* tensors_host, int64_t n, int64_t* step, double lr,
+                                 const float* lr_device, double beta1, double beta2, double eps, double weight_decay,
+                                 const float* norm, double max_norm, void* stream);
+
 /* Number of kernels the last flexsae_loss_fwd / flexsae_loss_bwd call of this thread enqueued
  * (for launch accounting in benchmarks). No reference counterpart. */
 int flexsae_last_launch_count(void);

@@ -1,0 +1,817 @@
+"""The optimizer operators: oracle pinned to torch and to its own definition on CPU, refusals, GPU parity.
+
+Tolerances.  u = 2^-24 is the largest relative error of one 32-bit operation, and the constants b, 1 - b
+are rounded to 32 bits too.  With c g the clipped gradient (its factor is off by at most 4 u):
+    m = b1 m + (1 - b1) c g          off by at most   (2 + 1) u |b1 m| + (4 + 3 + 1) u |(1 - b1) c g|
+    v = b2 v + (1 - b2) (c g)^2      off by at most   (2 + 1) u b2 v + (8 + 4 + 1) u (1 - b2) (c g)^2
+    p = p d - rate m / (sqrt(v) root + eps)
+        d: 1 u, product 1 u, difference 1 u                                  ->  4 u |p|
+        rate, root: 4 u each (expm1f 1 ulp = 2 u, a division, a rounding), sqrt(v): half of v's plus 1 u,
+        product, sum, two divisions, difference 1 u each                     ->  24 u |step| + the step that m's error makes
+The tests allow these sums, plus half a spacing where a result is rounded to 16 bits.
+"""
+import ctypes
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from flexsae_b200 import _native as nv
+from flexsae_b200 import optim
+from oracle import optim_oracle as orc
+
+U = 2.0 ** -24
+HALF = {torch.float32: (0.0, 0.0), torch.bfloat16: (2.0 ** -8, 2.0 ** -134), torch.float16: (2.0 ** -11, 2.0 ** -25)}
+gpu = pytest.mark.gpu
+
+
+# ---- CPU: the oracle --------------------------------------------------------------------------------
+def test_oracle_is_torchs_adamw():
+    g = torch.Generator().manual_seed(0)
+    p = torch.randn(40, 7, generator=g, dtype=torch.float64, requires_grad=True)
+    opt = torch.optim.AdamW([p], lr=3e-3, betas=(0.8, 0.95), eps=1e-6, weight_decay=0.1)
+    q, m, v = p.detach().numpy().copy(), np.zeros((40, 7)), np.zeros((40, 7))
+    for t in range(1, 6):
+        p.grad = torch.randn(40, 7, generator=g, dtype=torch.float64)
+        opt.step()
+        q, m, v = orc.adamw(q, p.grad.numpy(), m, v, t, 3e-3, (0.8, 0.95), 1e-6, 0.1)
+        np.testing.assert_allclose(p.detach().numpy(), q, rtol=1e-12, atol=1e-14)
+
+
+def test_oracle_keeps_rows_at_unit_length_and_steps_across_them():
+    r = np.random.default_rng(0)
+    w = r.standard_normal((5, 12))
+    w /= np.linalg.norm(w, axis=1, keepdims=True)
+    w[3] = 0
+    p, m, _ = orc.adamw(w, r.standard_normal((5, 12)), np.zeros((5, 12)), np.zeros((5, 12)), 1, 1e-2, unit_rows=True)
+    np.testing.assert_allclose(np.linalg.norm(p, axis=1), 1, rtol=1e-14)
+    np.testing.assert_allclose(np.sum(m * w, axis=1), 0, atol=1e-15)         # the gradient across its row
+
+
+@pytest.mark.parametrize("kind,dtype", [("m", torch.float8_e4m3fn), ("v", torch.float8_e5m2)])
+def test_oracle_formats_are_torchs(kind, dtype):
+    c = np.arange(256, dtype=np.uint8)
+    if kind == "v":
+        c = c[(c & 0x7F) < 0x7C]
+    want = torch.from_numpy(c).view(dtype).float().numpy()
+    np.testing.assert_array_equal(orc.widen(c, kind), want)
+
+
+@pytest.mark.parametrize("kind,largest", [("m", 448.0), ("v", 57344.0)])
+def test_oracle_rounding_is_right_on_average(kind, largest):
+    """Every value goes to one of its two neighbours, upwards with the right probability: over all 2^k random
+    numbers the mean is the value, up to the last bits that the random number has no room for (2^-20 of a spacing) and
+    the rounding of x / scale (2 u)."""
+    r = np.random.default_rng(1)
+    x = (r.standard_normal(256) * 10.0 ** r.uniform(-6, 0, 256)).astype(np.float32)
+    if kind == "v":
+        x = np.abs(x)
+    s = orc.scales(x, largest)
+    bits = 20 if kind == "m" else 21
+    grid = orc.E4M3 if kind == "m" else orc.E5M2
+    y = np.abs(x.astype(np.float64) / s[0])
+    if kind == "v":
+        y = np.maximum(y, grid[1])
+    lower = grid[np.searchsorted(grid, y, side="right") - 1]
+    upper = grid[np.minimum(np.searchsorted(grid, y, side="right"), len(grid) - 1)]
+    n = 1024
+    total = np.zeros(256)
+    for k in range(n):                              # random numbers spread evenly: the mean is exact to 1 / n of a spacing
+        c = orc.codes(x, s, np.full(256, (k << bits) // n), kind)
+        q = np.abs(orc.widen(c, kind).astype(np.float64))
+        assert np.all((q == lower) | (q == upper))
+        total += q
+    assert np.all(np.abs(total / n - y) <= (upper - lower) / n + 2 * U * y)
+
+
+def test_second_moment_follows_a_change_that_rounding_to_nearest_would_not_show():
+    """The reason for the random rounding: gradients of size 1 for 100 steps, then of size 0.1 beside one of size
+    1 that holds the scale.  After 3000 steps the average of v is 0.01 + (v0 - 0.01) * 0.999^3000, with v0 what the
+    first codes stand for (cut off without random bits, 1 becomes the second largest code, 6/7); 2048 elements are
+    averaged, each within about 75 % of it, so their mean is within 6 % (4 standard deviations of 0.75 / sqrt(2040)).
+    To nearest it stays where it was, since a step moves it by 0.1 % and the spacing is 12 to 25 %."""
+    n, b2 = 2048, np.float32(0.999)
+    g = np.ones(n, dtype=np.float32)
+    small = np.where(np.arange(n) % 256 == 0, 1.0, 0.1).astype(np.float32)
+    start = orc.scales(np.ones(n, dtype=np.float32), 57344.0)
+    v8, s = orc.codes(np.ones(n, dtype=np.float32), start, np.zeros(n, dtype=np.int64), "v"), start
+    nearest, s_near = v8.copy(), s.copy()
+    quiet = np.arange(n) % 256 != 0
+    v0 = float((orc.widen(v8, "v") * np.repeat(s, 256))[1])
+    assert abs(v0 - 6 / 7) < 1e-5
+    r = np.random.default_rng(2)
+    for _ in range(3000):
+        step = lambda c, sc: b2 * (orc.widen(c, "v") * np.repeat(sc, 256)) + np.float32(0.001) * small * small  # noqa: E731
+        v = step(v8, s)
+        s = orc.scales(v, 57344.0)
+        v8 = orc.codes(v, s, r.integers(0, 2 ** 21, n), "v")
+        v = step(nearest, s_near)
+        s_near = orc.scales(v, 57344.0)
+        nearest = orc.codes(v, s_near, np.full(n, 2 ** 20), "v")
+    got = (orc.widen(v8, "v") * np.repeat(s, 256))[quiet].mean()
+    want = 0.01 + (v0 - 0.01) * 0.999 ** 3000
+    assert abs(got - want) < 0.06 * want
+    assert (orc.widen(nearest, "v") * np.repeat(s_near, 256))[quiet].mean() > 0.5
+
+
+# ---- CPU: refusals ------------------------------------------------------------------------------------
+def _entry(n=1, rows=False, bits=32, lr=1e-3, lr_dev=None, betas=(0.9, 0.999), eps=1e-8, wd=0.0, norm=None, max_norm=1.0, step=512,
+           count=None, table=True, **tensor):
+    """Calls a step's C entry with addresses that nothing may touch; every such call has to be refused."""
+    lib = nv.load()
+    words = dict(param=1 << 20, grad=2 << 20, m=3 << 20, v=4 << 20, ms=5 << 20, vs=6 << 20, master=0, numel=512, cols=256,
+                 pdt=nv.F32, gdt=nv.F32)
+    rows_of = []
+    for i in range(n):
+        w = {**words, **{k: (x[i] if isinstance(x, (list, tuple)) else x) for k, x in tensor.items()}}
+        for k in ("param", "grad", "m", "v", "ms", "vs"):       # tensors of their own, unless the case places them
+            if k not in tensor:
+                w[k] += i << 24
+        rows_of += [w["param"], w["grad"], w["m"], w["v"], w["ms"], w["vs"], w["master"], w["numel"], w["cols"], w["pdt"] | w["gdt"] << 32]
+    t = (ctypes.c_int64 * max(1, len(rows_of)))(*rows_of) if table else None
+    count = n if count is None else count
+    if rows:
+        rc = lib.flexsae_adamw_unit_rows_step(t, count, step, lr, lr_dev, *betas, eps, wd, norm, max_norm, None)
+    else:
+        rc = lib.flexsae_adamw_step(t, count, bits, step, lr, lr_dev, *betas, eps, wd, norm, max_norm, 0, None)
+    return rc, lib.flexsae_last_error().decode()
+
+
+@pytest.mark.parametrize("kw,text", [
+    (dict(step=None), "step"), (dict(step=516), "aligned"), (dict(bits=16), "16 bits"),
+    (dict(lr=-1.0), "lr"), (dict(lr=math.inf), "lr"), (dict(lr=math.nan), "lr"),
+    (dict(betas=(1.0, 0.9)), "betas"), (dict(betas=(0.9, -0.1)), "betas"), (dict(betas=(math.nan, 0.9)), "betas"),
+    (dict(eps=0.0), "eps"), (dict(eps=1e-40), "eps"), (dict(eps=math.inf), "eps"), (dict(wd=-1.0), "weight_decay"),
+    (dict(norm=64, max_norm=0.0), "max_norm"), (dict(norm=64, max_norm=math.nan), "max_norm"),
+    (dict(count=-1), "tensors"), (dict(count=1 << 20), "tensors"), (dict(table=False), "null"),
+    (dict(param=0), "null"), (dict(grad=0), "null"), (dict(m=0), "null"), (dict(v=0), "null"),
+    (dict(bits=8, ms=0), "scales"), (dict(bits=8, vs=0), "scales"),
+    (dict(numel=-1), "numel"), (dict(numel=1 << 41), "numel"), (dict(pdt=7), "dtype"), (dict(pdt=nv.BF16, gdt=nv.F16), "gradient"),
+    (dict(pdt=nv.F32, gdt=nv.BF16), "gradient"), (dict(master=7 << 20), "master"),
+    (dict(param=(1 << 20) + 2), "aligned"), (dict(pdt=nv.BF16, grad=(2 << 20) + 2), "aligned"), (dict(pdt=nv.BF16, gdt=nv.BF16, param=(1 << 20) + 1), "aligned"),
+    (dict(pdt=nv.BF16, master=(7 << 20) + 2), "aligned"), (dict(bits=8, ms=(5 << 20) + 1), "aligned"),
+    (dict(grad=1 << 20), "overlap"), (dict(m=(4 << 20) - 4), "overlap"), (dict(bits=8, m=(4 << 20) - 511), "overlap"),
+    (dict(bits=8, vs=(5 << 20) + 4), "overlap"), (dict(n=2, param=1 << 20, m=[3 << 20, 7 << 20], v=[4 << 20, 8 << 20]), "twice"),
+    (dict(n=2, m=3 << 20), "overlap"), (dict(n=40, v=4 << 20), "overlap"),
+    (dict(rows=True, cols=0), "rows"), (dict(rows=True, cols=200), "rows"), (dict(rows=True, numel=16384, cols=16384), "8192"),
+])
+def test_step_entries_refuse_before_any_launch(kw, text):
+    rc, err = _entry(**kw)
+    assert rc < 0 and text in err, (rc, err)
+
+
+def test_norm_entry_refuses_before_any_launch():
+    lib = nv.load()
+    need = lib.flexsae_grad_norm_workspace_bytes(2)
+    assert need > 0 and lib.flexsae_grad_norm_workspace_bytes(-1) == 0 and lib.flexsae_grad_norm_workspace_bytes(1 << 17) == 0
+
+    def call(grads=(64, 128), numel=(4, 4), dtypes=(0, 1), n=2, out=512, ws=1024, ws_bytes=need):
+        return lib.flexsae_grad_norm((ctypes.c_void_p * 2)(*grads), (ctypes.c_int64 * 2)(*numel), (ctypes.c_int32 * 2)(*dtypes), n, out, ws,
+                                     ws_bytes, None), lib.flexsae_last_error().decode()
+
+    for kw, text in ((dict(n=-1), "tensors"), (dict(out=None), "null"), (dict(ws=None), "null"), (dict(ws=1028), "aligned"),
+                     (dict(ws_bytes=need - 1), "too small"), (dict(dtypes=(0, 5)), "dtype"), (dict(numel=(4, -4)), "numel"),
+                     (dict(grads=(64, 0)), "null"), (dict(grads=(66, 128)), "aligned"), (dict(grads=(64, 129)), "aligned")):
+        rc, err = call(**kw)
+        assert rc < 0 and text in err, (kw, rc, err)
+    assert lib.flexsae_grad_norm(None, None, None, 2, 512, 1024, need, None) == -1
+
+
+def test_python_entries_need_cuda_tensors():
+    p, step = torch.zeros(8), torch.zeros((), dtype=torch.int64)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        optim.adamw_step([p], [p.clone()], [p.clone()], [p.clone()], step, lr=1e-3)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        optim.grad_norm([p])
+    with pytest.raises(ValueError):
+        optim.grad_norm([])
+    with pytest.raises(ValueError):
+        optim.adamw_step([], [], [], [], step, lr=1e-3)
+    with pytest.raises(ValueError, match="gradients"):
+        optim.adamw_step([p], [], [p], [p], step, lr=1e-3)
+
+
+def test_optimizer_class_refuses_what_it_cannot_do():
+    p, q = torch.nn.Parameter(torch.zeros(4, 8)), torch.nn.Parameter(torch.zeros(8))
+    for bad in (dict(state_bits=16), dict(state_bits=8, unit_rows=True), dict(max_norm=0.0), dict(max_norm=-1.0)):
+        with pytest.raises(ValueError):
+            optim.AdamW([p], **bad)
+    with pytest.raises(ValueError, match="unit rows"):
+        optim.AdamW([q], unit_rows=True)
+    with pytest.raises(TypeError):
+        optim.AdamW([torch.nn.Parameter(torch.zeros(4, dtype=torch.float64))])
+    opt = optim.AdamW([p], unit_rows=True)
+    with pytest.raises(ValueError):
+        opt.add_param_group({"params": [q], "unit_rows": True})
+    assert len(opt.param_groups) == 1                              # a refused group is not kept
+
+
+# ---- GPU: helpers ---------------------------------------------------------------------------------------
+def f64(t):
+    return t.detach().double().cpu().numpy()
+
+
+def steps_in(name):
+    return torch.tensor(name, dtype=torch.int64, device="cuda")
+
+
+def make(shape, dtype, seed, master=False, grad_dtype=None, offset=0, spread=True):
+    """(p, g, m, v, master) on the GPU, optionally ``offset`` elements into their storage; some gradients are zero."""
+    g = torch.Generator().manual_seed(seed)
+    n = math.prod(shape)
+
+    def place(x, dt):
+        store = torch.zeros(n + offset, dtype=dt, device="cuda")
+        return store[offset:].view(shape).copy_(x)
+
+    p = torch.randn(shape, generator=g)
+    grad = torch.randn(shape, generator=g) * 1e-2
+    if spread:
+        grad = grad * 10.0 ** (torch.rand(shape, generator=g) * 3 - 2)
+    grad[torch.rand(shape, generator=g) < 0.1] = 0
+    m, v = torch.randn(shape, generator=g) * 3e-3, torch.randn(shape, generator=g).square() * 1e-5
+    return (place(p, dtype), place(grad, grad_dtype or dtype), place(m, torch.float32), place(v, torch.float32),
+            place(p, torch.float32) if master else None)
+
+
+def bounds(before, after, t, lr, betas, eps, clip):
+    """Allowed errors of (p, m, v), see the head of this file; ``after`` is the oracle's answer."""
+    p, g, m, v = (np.abs(x) for x in before)
+    g = g * clip
+    em = U * (3 * betas[0] * m + 8 * (1 - betas[0]) * g)
+    ev = U * (3 * betas[1] * v + 13 * (1 - betas[1]) * g * g)
+    denom = np.sqrt(after[2]) / math.sqrt(1 - betas[1] ** t) + eps
+    rate = lr / (1 - betas[0] ** t)
+    relative_v = np.divide(ev, after[2], out=np.zeros_like(ev), where=after[2] > 0) / 2
+    step = rate * np.abs(after[1]) / denom
+    return 4 * U * p + (24 * U + relative_v) * step + rate * em / denom, em + 2.0 ** -149, ev + 2.0 ** -148
+
+
+def close(got, want, bound, what):
+    bad = ~(np.abs(f64(got) - want) <= bound)
+    assert not bad.any(), (what, int(bad.sum()), np.abs(f64(got) - want)[bad][:4], np.broadcast_to(bound, bad.shape)[bad][:4])
+
+
+def check_params(p, master, want, bound, dtype):
+    half, tiny = HALF[dtype]
+    close(p, want, bound + half * np.abs(want) + half * bound + tiny, "param")
+    if master is not None:
+        close(master, want, bound, "master")
+        assert torch.equal(p, master.to(dtype))                     # the parameter is its copy, rounded
+
+
+# ---- GPU: gradient norm ------------------------------------------------------------------------------------
+# 32-bit sums of eight squares (8 u), then 64 bits; the root halves that and the result is rounded: 5 u
+NORM_TOL = 5 * U
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n,offset", [(1, 0), (7, 0), (255, 1), (256, 0), (257, 3), (8191, 0), (8192, 0), (8193, 1), (100003, 0), (20_000_001, 0)])
+def test_norm_of_one_tensor(dtype, n, offset):
+    x = torch.randn(n + offset, generator=torch.Generator().manual_seed(n)).to(dtype).cuda()[offset:]
+    want = float(x.double().square().sum().sqrt())
+    got = optim.grad_norm([x])
+    assert got.dtype == torch.float32 and got.shape == () and abs(float(got) - want) <= NORM_TOL * want
+    assert torch.equal(got, optim.grad_norm([x]))
+
+
+@gpu
+@pytest.mark.parametrize("count", [2, 16, 17, 256, 257, 600])
+def test_norm_of_many_mixed_tensors(count):
+    g = torch.Generator().manual_seed(count)
+    dtypes = [torch.float32, torch.bfloat16, torch.float16]
+    xs = [torch.randn((i * 37) % 501, generator=g).to(dtypes[i % 3]).cuda() for i in range(count)]
+    xs.append(torch.randn(50, 60, generator=g).cuda().t())                              # dense, another order
+    xs.append(torch.randn(50, 60, generator=g).cuda()[:, ::2])                         # with gaps
+    want = math.sqrt(sum(float(x.double().square().sum()) for x in xs))
+    assert abs(float(optim.grad_norm(xs)) - want) <= NORM_TOL * want
+
+
+@gpu
+def test_norm_of_extreme_values():
+    big = torch.full((1000,), 1e30, device="cuda")
+    assert abs(float(optim.grad_norm([big])) - float(big[0]) * math.sqrt(1000)) <= NORM_TOL * 1e30 * 32
+    small = torch.full((1000,), 1e-30, device="cuda")
+    small[::3] = 0
+    assert abs(float(optim.grad_norm([small])) - float(small.double().square().sum().sqrt())) <= NORM_TOL * 1e-28
+    assert float(optim.grad_norm([torch.zeros(5000, device="cuda")])) == 0
+    assert float(optim.grad_norm([torch.empty(0, device="cuda")])) == 0
+    for bad in (math.inf, -math.inf):
+        big[17] = bad
+        assert float(optim.grad_norm([small, big])) == math.inf
+    big[18] = math.nan
+    assert math.isnan(float(optim.grad_norm([small, big])))
+
+
+# ---- GPU: AdamW, 32-bit states ------------------------------------------------------------------------
+KINDS = [(torch.float32, torch.float32, False)] + [(d, g, m) for d in (torch.bfloat16, torch.float16)
+                                                   for g in (d, torch.float32) for m in (False, True)]
+SHAPES = [(1,), (3,), (255,), (256,), (257,), (2047,), (2049,), (1, 4096), (61, 77), (1000, 129)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("t", [1, 1000])
+def test_adamw_against_the_oracle(dtype, grad_dtype, master, offset, t):
+    sets = [make(s, dtype, 100 * k + offset, master, grad_dtype, offset) for k, s in enumerate(SHAPES)]
+    if t == 1:
+        for x in sets:
+            x[2].zero_(), x[3].zero_()
+    before = [[f64(x[4] if master else x[0]), f64(x[1]), f64(x[2]), f64(x[3])] for x in sets]
+    kw = dict(lr=3e-3, betas=(0.9, 0.99), eps=1e-6, weight_decay=0.1)
+    step = steps_in(t - 1)
+    optim.adamw_step(*[[x[k] for x in sets] for k in range(4)], step, masters=[x[4] for x in sets] if master else None, **kw)
+    assert int(step) == t
+    for x, b in zip(sets, before):
+        want = orc.adamw(*b, t, 3e-3, (0.9, 0.99), 1e-6, 0.1)
+        ep, em, ev = bounds(b, want, t, 3e-3, (0.9, 0.99), 1e-6, 1.0)
+        check_params(x[0], x[4], want[0], ep, dtype)
+        close(x[2], want[1], em, "m")
+        close(x[3], want[2], ev, "v")
+
+
+@gpu
+def test_adamw_on_many_tensors_of_all_kinds_with_empty_ones():
+    """Over 256 tensors of one kind, every other kind beside them, empty tensors among them: every element is updated
+    once and the count moves by one."""
+    sets, masters = [], []
+    for i in range(330):
+        dtype, grad_dtype, master = KINDS[0] if i < 300 else KINDS[i % len(KINDS)]
+        x = make(((i * 131) % 700,), dtype, i, master, grad_dtype)
+        sets.append(x)
+        masters.append(x[4])
+    before = [[f64(x[4] if x[4] is not None else x[0]), f64(x[1]), f64(x[2]), f64(x[3])] for x in sets]
+    step = steps_in(4)
+    optim.adamw_step(*[[x[k] for x in sets] for k in range(4)], step, lr=1e-3, masters=masters)
+    assert int(step) == 5
+    for x, b in zip(sets, before):
+        want = orc.adamw(*b, 5, 1e-3)
+        ep, em, ev = bounds(b, want, 5, 1e-3, (0.9, 0.999), 1e-8, 1.0)
+        check_params(x[0], x[4], want[0], ep, x[0].dtype)
+        close(x[2], want[1], em, "m")
+        close(x[3], want[2], ev, "v")
+
+
+@gpu
+def test_only_empty_tensors_still_count_the_step():
+    e, step = [torch.empty(0, device="cuda") for _ in range(4)], steps_in(7)
+    optim.adamw_step(*[[x] for x in e], step, lr=1e-3)
+    assert int(step) == 8
+    e = [torch.empty(0, 8, device="cuda") for _ in range(4)]
+    optim.adamw_unit_rows_step(*[[x] for x in e], step, lr=1e-3)
+    assert int(step) == 9
+
+
+@gpu
+@pytest.mark.parametrize("max_norm", [0.25, 1e9])
+def test_clipping_uses_the_norm_on_the_device(max_norm):
+    x = make((300, 70), torch.float32, 5)
+    b = [f64(t) for t in x[:4]]
+    norm = optim.grad_norm([x[1]])
+    step = steps_in(9)
+    optim.adamw_step(*[[t] for t in x[:4]], step, lr=1e-2, norm=norm, max_norm=max_norm)
+    clip = orc.clip_factor(float(norm), max_norm)
+    assert clip < 1 if max_norm < 1 else clip == 1
+    want = orc.adamw(*b, 10, 1e-2, clip=clip)
+    ep, em, ev = bounds(b, want, 10, 1e-2, (0.9, 0.999), 1e-8, clip)
+    close(x[0], want[0], ep, "param"), close(x[2], want[1], em, "m"), close(x[3], want[2], ev, "v")
+
+
+@gpu
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("entry", ["adamw", "adamw8", "rows"])
+def test_a_norm_that_is_not_finite_leaves_everything(bad, entry):
+    x, step, norm = make((40, 64), torch.bfloat16, 6, master=True), steps_in(3), torch.tensor(bad, device="cuda")
+    m, v = x[2], x[3]
+    if entry == "adamw8":
+        m, v = (torch.randint(0, 100, (40, 64), dtype=torch.uint8, device="cuda").view(d) for d in optim.STATE8_DTYPES)
+    scales = [torch.rand(10, device="cuda") for _ in range(2)]
+    state = [x[0], x[4], m.view(torch.uint8), v.view(torch.uint8), *scales, step]
+    kept = [t.clone() for t in state]
+    kw = dict(lr=1e-3, norm=norm, masters=[x[4]])
+    if entry == "adamw8":
+        optim.adamw8_step([x[0]], [x[1]], [m], [scales[0]], [v], [scales[1]], step, max_norm=1.0, **kw)
+    else:
+        (optim.adamw_step if entry == "adamw" else optim.adamw_unit_rows_step)([x[0]], [x[1]], [m], [v], step, **kw)
+    for a, b in zip(state, kept):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_nonfinite_gradients_without_a_norm_stay_with_their_elements():
+    x = make((1000,), torch.float32, 7)
+    y = [t.clone() for t in x[:4]]
+    x[1][123], x[1][700] = math.nan, math.inf
+    optim.adamw_step(*[[t] for t in x[:4]], steps_in(0), lr=1e-3)
+    optim.adamw_step(*[[t] for t in y], steps_in(0), lr=1e-3)
+    keep = torch.ones(1000, dtype=torch.bool, device="cuda")
+    keep[[123, 700]] = False
+    for a, b in zip((x[0], x[2], x[3]), (y[0], y[2], y[3])):
+        assert torch.equal(a[keep], b[keep]) and not torch.isfinite(a[~keep]).any()
+
+
+@gpu
+def test_layouts_transposed_parameters_and_foreign_gradients():
+    """A transposed parameter with states like it; a gradient in another order is brought into it."""
+    p, g, m, v, _ = make((48, 80), torch.float32, 8)
+    b = [f64(t) for t in (p, g, m, v)]
+    pt, mt, vt = (torch.empty(80, 48, device="cuda").t().copy_(t) for t in (p, m, v))
+    step = steps_in(0)
+    optim.adamw_step([pt], [g], [mt], [vt], step, lr=1e-3)
+    want = orc.adamw(*b, 1, 1e-3)
+    ep, em, ev = bounds(b, want, 1, 1e-3, (0.9, 0.999), 1e-8, 1.0)
+    close(pt, want[0], ep, "param"), close(mt, want[1], em, "m"), close(vt, want[2], ev, "v")
+
+
+@gpu
+def test_python_refusals_on_cuda_tensors():
+    p, g, m, v, _ = make((16, 32), torch.bfloat16, 9)
+    step = steps_in(0)
+
+    def call(p=p, g=g, m=m, v=v, step=step, **kw):
+        optim.adamw_step([p], [g], [m], [v], step, **{**dict(lr=1e-3), **kw})
+
+    for err, kw in (
+            (TypeError, dict(p=p.double(), g=g.double())), (TypeError, dict(g=g.half())), (TypeError, dict(g=g.to_sparse())),
+            (TypeError, dict(m=m.bfloat16())), (TypeError, dict(step=step.int())), (TypeError, dict(norm=torch.zeros((), device="cuda", dtype=torch.float64))),
+            (ValueError, dict(g=g[:8])), (ValueError, dict(m=m[:8])), (ValueError, dict(m=m.t().contiguous().t())),
+            (ValueError, dict(p=torch.zeros(16, 64, device="cuda")[:, ::2], g=g.float())), (ValueError, dict(step=torch.zeros(2, dtype=torch.int64, device="cuda"))),
+            (ValueError, dict(lr=-1.0)), (ValueError, dict(betas=(0.9, 1.0))), (ValueError, dict(eps=0.0)), (ValueError, dict(weight_decay=math.nan)),
+            (ValueError, dict(max_norm=1.0)), (ValueError, dict(norm=torch.zeros((), device="cuda"), max_norm=0.0)),
+            (ValueError, dict(p=p.float(), g=g.float(), masters=[m.clone()])), (ValueError, dict(masters=[])), (RuntimeError, dict(m=m.cpu())),
+            (RuntimeError, dict(g=g.cpu())), (RuntimeError, dict(step=step.cpu())), (nv.FlexSaeNativeError, dict(v=m))):
+        kept = [t.clone() for t in (p, m, v, step)]
+        with pytest.raises(err):
+            call(**kw)
+        assert all(torch.equal(a, b) for a, b in zip((p, m, v, step), kept))
+    with pytest.raises(nv.FlexSaeNativeError, match="twice"):
+        optim.adamw_step([p, p], [g, g], [m, m.clone()], [v, v.clone()], step, lr=1e-3)
+    with pytest.raises(ValueError):
+        optim.adamw_unit_rows_step([p.t()], [g.t()], [m.t()], [v.t()], step, lr=1e-3)
+    with pytest.raises(ValueError):
+        optim.adamw_unit_rows_step([p[0]], [g[0]], [m[0]], [v[0]], step, lr=1e-3)
+    with pytest.raises(ValueError, match="seed"):
+        optim.adamw8_step([p], [g], [m.to(torch.float8_e4m3fn)], [torch.zeros(2, device="cuda")], [v.to(torch.float8_e5m2)],
+                          [torch.zeros(2, device="cuda")], step, lr=1e-3, seed=-1)
+    with pytest.raises(ValueError, match="scales"):
+        optim.adamw8_step([p], [g], [m.to(torch.float8_e4m3fn)], [torch.zeros(3, device="cuda")], [v.to(torch.float8_e5m2)],
+                          [torch.zeros(2, device="cuda")], step, lr=1e-3)
+
+
+# ---- GPU: 8-bit states ----------------------------------------------------------------------------------
+def make8(shape, dtype, seed, master=False, offset=0):
+    p, g, m, v, w = make(shape, dtype, seed, master, offset=offset)
+    n = p.numel()
+    state = []
+    for x, kind, largest, dt in ((m, "m", 448.0, torch.float8_e4m3fn), (v, "v", 57344.0, torch.float8_e5m2)):
+        flat = x.reshape(-1).cpu().numpy()
+        s = orc.scales(flat, largest)
+        c = orc.codes(flat, s, np.full(n, 1 << 19), kind)
+        store = torch.zeros(n + offset, dtype=torch.uint8, device="cuda")
+        store[offset:] = torch.from_numpy(c)
+        state += [store[offset:].view(dt).view(shape), torch.from_numpy(s).cuda()]
+    return [p, g, *state, w]
+
+
+def bytes_of(t):
+    return t.view(torch.uint8).reshape(-1).cpu().numpy()
+
+
+@gpu
+@pytest.mark.parametrize("dtype,master", [(torch.float32, False), (torch.bfloat16, False), (torch.bfloat16, True), (torch.float16, True)])
+@pytest.mark.parametrize("offset", [0, 1])
+@pytest.mark.parametrize("clipped", [False, True])
+def test_adamw8_states_are_the_oracles_bits(dtype, master, offset, clipped):
+    """Moments, scales and codes bit for bit as the definition in 32-bit arithmetic gives them; the parameter within
+    the bounds of its formula, from the moments before their rounding.  Three steps in a row."""
+    sets = [make8(s, dtype, 10 * k, master, offset) for k, s in enumerate(SHAPES)]
+    step = steps_in(40)
+    norm = torch.tensor(3.0, device="cuda") if clipped else None
+    f = np.float32
+    clip = min(f(1) / (f(3.0) + f(1e-6)) * f(0.7), f(1)) if clipped else f(1)
+    for k in range(3):
+        before = [[f64(x[6] if master else x[0]), x[1].float().cpu().numpy().reshape(-1), bytes_of(x[2]), x[3].cpu().numpy(), bytes_of(x[4]),
+                   x[5].cpu().numpy()] for x in sets]
+        optim.adamw8_step(*[[x[j] for x in sets] for j in range(6)], step, lr=2e-3, eps=1e-6, masters=[x[6] for x in sets] if master else None,
+                          norm=norm, max_norm=0.7 if clipped else None, seed=77)
+        assert int(step) == 41 + k
+        for i, (x, b) in enumerate(zip(sets, before)):
+            m, v, m8, ms, v8, vs = orc.adamw8_states(*b[1:], 41 + k, 77, i, clip=clip)
+            assert np.array_equal(x[3].cpu().numpy(), ms) and np.array_equal(x[5].cpu().numpy(), vs)
+            assert np.array_equal(bytes_of(x[2]), m8) and np.array_equal(bytes_of(x[4]), v8)
+            shape = tuple(x[0].shape)
+            m, v = m.reshape(shape).astype(np.float64), v.reshape(shape).astype(np.float64)
+            t, p = 41 + k, b[0].reshape(shape)
+            rate, denom = 2e-3 / (1 - 0.9 ** t), np.sqrt(v) / math.sqrt(1 - 0.999 ** t) + 1e-6
+            want = p * (1 - 2e-3 * 0.01) - rate * m / denom
+            check_params(x[0], x[6], want, 4 * U * np.abs(p) + 32 * U * rate * np.abs(m) / denom, dtype)
+
+
+@gpu
+def test_adamw8_from_zero_states_and_idle_blocks():
+    """First step from nothing; a block without any gradient keeps scales of zero and codes that widen to zero."""
+    p = torch.randn(1024, device="cuda")
+    g = torch.randn(1024, device="cuda")
+    g[256:512] = 0
+    p0 = p.clone()
+    m, v = torch.zeros(1024, dtype=torch.float8_e4m3fn, device="cuda"), torch.zeros(1024, dtype=torch.float8_e5m2, device="cuda")
+    sm, sv, step = torch.zeros(4, device="cuda"), torch.zeros(4, device="cuda"), steps_in(0)
+    optim.adamw8_step([p], [g], [m], [sm], [v], [sv], step, lr=1e-3, weight_decay=0.0)
+    assert torch.equal(p[256:512], p0[256:512]) and float(sm[1]) == 0 and float(sv[1]) == 0
+    sure = g.abs() > 1e-4                                              # eps = 1e-8 takes 1e-4 of the step at most
+    sure[256:512] = False
+    assert torch.allclose((p0 - p)[sure], 1e-3 * torch.sign(g[sure]), rtol=2e-3, atol=0)
+    widened = m.float() * sm.repeat_interleave(256)
+    assert bool(((widened - 0.1 * g).abs() <= 0.125 * (0.1 * g).abs() + sm.repeat_interleave(256) * 2.0 ** -9 + 1e-9).all())
+
+
+@gpu
+def test_adamw8_nonfinite_values_stay_with_their_elements():
+    sets = [make8((768,), torch.float32, 11) for _ in range(2)]
+    sets[0][1][300], sets[0][1][301] = math.nan, math.inf
+    before = [sets[0][1].cpu().numpy(), bytes_of(sets[0][2]), sets[0][3].cpu().numpy(), bytes_of(sets[0][4]), sets[0][5].cpu().numpy()]
+    for x in sets:
+        optim.adamw8_step(*[[x[j]] for j in range(6)], steps_in(0), lr=1e-3, seed=3)
+    _, _, m8, ms, v8, vs = orc.adamw8_states(*before, 1, 3, 0)
+    x = sets[0]
+    assert np.array_equal(bytes_of(x[2]), m8) and np.array_equal(bytes_of(x[4]), v8)
+    assert np.array_equal(x[3].cpu().numpy(), ms) and np.array_equal(x[5].cpu().numpy(), vs)
+    keep = torch.ones(768, dtype=torch.bool, device="cuda")
+    keep[[300, 301]] = False
+    assert torch.equal(x[0][keep], sets[1][0][keep]) and not torch.isfinite(x[0][~keep]).any()
+    assert torch.isnan(x[2].float()[[300, 301]]).all() and torch.isnan(x[4].float()[[300, 301]]).all()
+
+
+@gpu
+@pytest.mark.parametrize("scale", [1e-22, 1e15])
+def test_adamw8_extreme_gradients(scale):
+    """Squares near the ends of the 32-bit range: tiny blocks fall to a scale of zero, large ones stay finite."""
+    x = make8((512,), torch.float32, 12)
+    x[1].copy_(torch.randn(512, generator=torch.Generator().manual_seed(1)) * scale)
+    for k in (2, 4):
+        x[k].view(torch.uint8).zero_()
+        x[k + 1].zero_()
+    before = [x[1].cpu().numpy(), bytes_of(x[2]), x[3].cpu().numpy(), bytes_of(x[4]), x[5].cpu().numpy()]
+    optim.adamw8_step(*[[x[j]] for j in range(6)], steps_in(0), lr=1e-3, seed=5)
+    _, _, m8, ms, v8, vs = orc.adamw8_states(*before, 1, 5, 0)
+    assert np.array_equal(bytes_of(x[2]), m8) and np.array_equal(bytes_of(x[4]), v8)
+    assert np.array_equal(x[3].cpu().numpy(), ms) and np.array_equal(x[5].cpu().numpy(), vs)
+    assert torch.isfinite(x[0]).all()
+
+
+# ---- GPU: unit rows -------------------------------------------------------------------------------------
+def rows_bounds(b, want, t, lr, clip):
+    """As ``bounds``, for the row form.  A sum over a row is off by at most (8 + 10 + 1) u of the sum of its absolute terms
+    (eight in a row, five and five levels of a tree), so the projection moves g by (40 u) |along|abs |p| + 3 u of its own terms;
+    a new row is divided by its length (12 u of the row, and the errors of its elements once more through the length)."""
+    p, g, m, v = b
+    g = g * clip
+    square = np.sum(p * p, axis=1, keepdims=True)
+    along = np.divide(np.sum(np.abs(g * p), axis=1, keepdims=True), square, out=np.zeros_like(square), where=square > 0)
+    eg = U * (48 * along * np.abs(p) + 8 * np.abs(g))
+    projected = np.abs(g) + along * np.abs(p)
+    em = U * (3 * 0.9 * np.abs(m) + 4 * 0.1 * projected) + 0.1 * eg
+    ev = U * (3 * 0.999 * np.abs(v) + 5 * 0.001 * projected ** 2) + 0.001 * (2 * projected * eg + eg * eg)
+    # errors of the step, to first order around the exact moments, the denominator at its smallest
+    denom = np.sqrt(np.maximum(want[2] - ev, 0)) / math.sqrt(1 - 0.999 ** t) + 1e-8
+    rate = lr / (1 - 0.9 ** t)
+    upper = np.sqrt(want[2] + ev) / math.sqrt(1 - 0.999 ** t) + 1e-8
+    ep = 4 * U * np.abs(p) + rate * (np.abs(want[1]) * (1 / denom - 1 / upper) + em / denom) + 24 * U * rate * np.abs(want[1]) / denom
+    new = p * (1 - lr * 0.01) - rate * want[1] / (np.sqrt(want[2]) / math.sqrt(1 - 0.999 ** t) + 1e-8)
+    length = np.sqrt(np.sum(new * new, axis=1, keepdims=True))
+    length = np.where(length > 0, length, 1)
+    through = np.sum(np.abs(want[0]) * ep, axis=1, keepdims=True) / length
+    return (ep / length + np.abs(want[0]) * (through + 12 * U)) * 1.01, em + 2.0 ** -149, ev + 2.0 ** -148
+
+
+@gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
+@pytest.mark.parametrize("F,D,offset", [(1, 1, 0), (5, 7, 0), (300, 8, 0), (33, 255, 0), (33, 256, 0), (33, 257, 1), (40, 512, 1), (500, 768, 0), (9, 2304, 0), (3, 8191, 0), (4, 8192, 0)])
+def test_unit_rows_against_the_oracle(dtype, grad_dtype, master, F, D, offset):
+    x = make((F, D), dtype, F + D, master, grad_dtype, offset, spread=False)
+    w = x[4] if master else x[0]
+    w.copy_(w.float() / w.float().norm(dim=1, keepdim=True))
+    if master:
+        x[0].copy_(w)
+    if F > 3:
+        w[1] = 0                                                # a row of zeros, a row without gradient
+        x[0][1] = 0
+        x[1][2] = 0
+    b = [f64(w), f64(x[1]), f64(x[2]), f64(x[3])]
+    step, norm = steps_in(20), torch.tensor(2.0, device="cuda")
+    optim.adamw_unit_rows_step(*[[t] for t in x[:4]], step, lr=1e-3, masters=[x[4]] if master else None, norm=norm, max_norm=1.0)
+    assert int(step) == 21
+    clip = orc.clip_factor(2.0, 1.0)
+    want = orc.adamw(*b, 21, 1e-3, clip=clip, unit_rows=True)
+    ep, em, ev = rows_bounds(b, want, 21, 1e-3, clip)
+    check_params(x[0], x[4], want[0], ep, dtype)
+    close(x[2], want[1], em, "m")
+    close(x[3], want[2], ev, "v")
+
+
+@gpu
+def test_unit_rows_of_several_decoders_and_zero_rows():
+    xs = [make(s, torch.float32, 60 + k, spread=False) for k, s in enumerate([(10, 64), (0, 64), (7, 1000), (3, 0)])]
+    for x in xs:
+        x[0].copy_(torch.nn.functional.normalize(x[0], dim=1))
+    xs[0][0][4], xs[0][1][4], xs[0][2][4], xs[0][3][4] = 0, 0, 0, 0
+    step = steps_in(2)
+    optim.adamw_unit_rows_step(*[[x[k] for x in xs] for k in range(4)], step, lr=1e-3)
+    assert int(step) == 3
+    assert float(xs[0][0][4].abs().max()) == 0
+    for x in (xs[0], xs[2]):
+        length = x[0].double().norm(dim=1)
+        assert bool(((length - 1).abs() <= 16 * U)[torch.arange(len(length), device="cuda") != (4 if x is xs[0] else -1)].all())
+    with pytest.raises(nv.FlexSaeNativeError, match="8192"):
+        y = make((2, 8200), torch.float32, 1)
+        optim.adamw_unit_rows_step(*[[t] for t in y[:4]], step, lr=1e-3)
+
+
+# ---- GPU: streams, graphs, versions --------------------------------------------------------------------
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps_replay_like_eager_ones(bits):
+    """The step count, the learning rate and the clipping factor are read on the device at every replay."""
+    def train(captured):
+        g = torch.Generator().manual_seed(3)
+        ps = [torch.nn.Parameter(torch.randn(s, generator=g).cuda()) for s in ((70, 33), (33,))]
+        lr = torch.tensor(1e-2, device="cuda")
+        opt = optim.AdamW(ps, lr=lr, state_bits=bits, max_norm=0.5)
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g).cuda()
+        graph = None
+        for k in range(6):
+            lr.fill_(1e-2 / (k + 1))
+            if captured and k == 2:
+                torch.cuda.synchronize()
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph):
+                    opt.step()
+            if graph is not None:
+                graph.replay()
+            else:
+                opt.step()
+            for p in ps:
+                p.grad.mul_(-0.7)
+        return [p.detach().clone() for p in ps] + [opt.state[ps[0]]["step"].clone()]
+
+    for a, b in zip(train(False), train(True)):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_steps_on_two_streams_do_not_disturb_each_other():
+    def run(streams):
+        sets = [make((4000, 257), torch.float32, 20 + k) for k in range(2)]
+        steps, norms = [steps_in(0), steps_in(0)], [None, None]
+        torch.cuda.synchronize()
+        for _ in range(5):
+            for k in range(2):
+                with torch.cuda.stream(streams[k]):
+                    norms[k] = optim.grad_norm([sets[k][1]])
+                    optim.adamw_step(*[[t] for t in sets[k][:4]], steps[k], lr=1e-3, norm=norms[k], max_norm=1.0)
+        torch.cuda.synchronize()
+        return [t for x in sets for t in (x[0], x[2], x[3])] + steps
+
+    one = torch.cuda.current_stream()
+    for a, b in zip(run([one, one]), run([torch.cuda.Stream(), torch.cuda.Stream()])):
+        assert torch.equal(a, b)
+
+
+@gpu
+def test_autograd_sees_that_a_parameter_changed():
+    p = torch.randn(8, device="cuda", requires_grad=True)
+    loss = (p * p).sum()
+    optim.adamw_step([p], [torch.ones(8, device="cuda")], [torch.zeros(8, device="cuda")], [torch.zeros(8, device="cuda")], steps_in(0), lr=1e-3)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+# ---- GPU: the optimizer class, and a training run -----------------------------------------------------------
+def make_sae(F, D, dtype, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    w = torch.nn.functional.normalize(torch.randn(F, D, generator=g), dim=1)
+    return {k: torch.nn.Parameter(t.to(dtype).cuda()) for k, t in
+            dict(w_enc=w.clone(), b_enc=torch.zeros(F), w_dec=w, b_dec=torch.zeros(D)).items()}
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("bits,master", [(32, False), (32, True), (8, False), (8, True)])
+def test_training_run_encoder_selection_loss_and_step(dtype, bits, master):
+    """Encoder, top-K selection, fused loss, its backward and the optimizer step together, four times: every step is what
+    the oracle makes of the gradients that the losses left, clipped by their norm, and the decoder's rows stay at
+    unit length."""
+    import flexsae_b200 as fx
+    from flexsae_b200 import producer
+
+    F, D, K, B, lr, max_norm = 512, 128, 16, 96, 1e-3, 0.05
+    sae = make_sae(F, D, dtype)
+    opt = optim.AdamW([{"params": [sae["w_enc"], sae["b_enc"], sae["b_dec"]], "state_bits": bits, "seed": 9},
+                       {"params": [sae["w_dec"]], "unit_rows": True}], lr=lr, eps=1e-6, max_norm=max_norm, master_weights=master)
+    held = master and dtype != torch.float32
+    m = {k: np.zeros(tuple(p.shape)) for k, p in sae.items()}
+    v = {k: np.zeros(tuple(p.shape)) for k, p in sae.items()}
+    for t in range(1, 5):
+        x = torch.randn(B, D, generator=torch.Generator().manual_seed(50 + t)).to(dtype).cuda()
+        idx, vals = producer.encode_topk(x - sae["b_dec"], sae["w_enc"], sae["b_enc"], K)
+        fx.triton_hierarchical_sae_loss(idx, sae["w_dec"], vals, sae["b_dec"], x).backward()
+        grads = {k: f64(p.grad) for k, p in sae.items()}
+        before = {k: f64(opt.state[p]["master"] if held and t > 1 else p) for k, p in sae.items()}
+        opt.step()
+        norm = math.sqrt(sum(float((g * g).sum()) for g in grads.values()))
+        assert abs(float(opt.norm) - norm) <= NORM_TOL * norm
+        clip = orc.clip_factor(float(opt.norm), max_norm)
+        for k, p in sae.items():
+            rows = k == "w_dec"
+            want = orc.adamw(before[k], grads[k], m[k], v[k], t, lr, eps=1e-6, clip=clip, unit_rows=rows)
+            state = opt.state[p]
+            assert int(state["step"]) == t
+            if rows or bits == 32:
+                b = (before[k], grads[k], m[k], v[k])
+                ep, em, ev = rows_bounds(b, want, t, lr, clip) if rows else bounds(b, want, t, lr, (0.9, 0.999), 1e-6, clip)
+                close(state["exp_avg"], want[1], em, k)
+                close(state["exp_avg_sq"], want[2], ev, k)
+                m[k], v[k] = f64(state["exp_avg"]), f64(state["exp_avg_sq"])
+            else:
+                # the parameter from moments off by the bounds above; here the 8-bit states are only read back
+                ep = bounds((before[k], grads[k], m[k], v[k]), want, t, lr, (0.9, 0.999), 1e-6, clip)[0]
+                m[k], v[k] = (f64(state[n].float().reshape(-1) * state[n + "_scale"].repeat_interleave(256)[: p.numel()]).reshape(tuple(p.shape))
+                              for n in ("exp_avg", "exp_avg_sq"))
+            check_params(p, state.get("master"), want[0], ep, dtype)
+        opt.zero_grad()
+    length = sae["w_dec"].double().norm(dim=1)
+    assert float((length - 1).abs().max()) <= (16 * U if dtype == torch.float32 else 2.0 ** -8)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dict_continues_the_run(bits):
+    def params():
+        return [torch.nn.Parameter(p.detach().clone()) for p in make_sae(64, 40, torch.bfloat16).values()]
+
+    def grads(ps, t):
+        g = torch.Generator().manual_seed(t)
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=g).to(p.dtype).cuda()
+
+    kw = dict(lr=1e-2, state_bits=bits, master_weights=True, seed=4)
+    a, b = params(), params()
+    first, second = optim.AdamW(a, **kw), optim.AdamW(b, **kw)
+    for t in range(3):
+        grads(a, t)
+        first.step()
+    with torch.no_grad():
+        for p, q in zip(a, b):
+            q.copy_(p)
+    second.load_state_dict(first.state_dict())
+    for p, q in zip(a, b):
+        for name, value in first.state[p].items():
+            assert second.state[q][name].dtype == value.dtype and second.state[q][name].data_ptr() != value.data_ptr()
+    for t in range(3, 5):
+        grads(a, t), grads(b, t)
+        first.step(), second.step()
+    assert len({id(second.state[q]["step"]) for q in b}) == 1
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for name, value in first.state[p].items():
+            assert torch.equal(value.view(torch.uint8) if value.dim() else value, second.state[q][name].view(torch.uint8) if value.dim() else second.state[q][name])
+
+
+@gpu
+def test_parameters_without_gradients_keep_their_own_count():
+    ps = [torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(3)]
+    opt = optim.AdamW(ps, lr=1e-2)
+    counts = [0, 0, 0]
+    for t, active in enumerate([(0, 1), (0, 1, 2), (1,), (0, 2), (0, 1, 2)]):
+        for k, p in enumerate(ps):
+            p.grad = torch.full_like(p, 0.1 * (t + 1)) if k in active else None
+        kept = [p.detach().clone() for p in ps]
+        opt.step()
+        for k, p in enumerate(ps):
+            counts[k] += k in active
+            assert torch.equal(p, kept[k]) == (k not in active)
+            assert (int(opt.state[p]["step"]) if opt.state.get(p) else 0) == counts[k]
+
+
+@gpu
+def test_skip_nonfinite_and_copies_of_the_optimizer():
+    import copy
+    import pickle
+
+    p = torch.nn.Parameter(torch.ones(300, device="cuda"))
+    opt = optim.AdamW([p], lr=1e-2, skip_nonfinite=True)
+    p.grad = torch.ones_like(p)
+    opt.step()
+    kept = p.detach().clone()
+    p.grad[7] = math.inf
+    opt.step()
+    assert torch.equal(p, kept) and int(opt.state[p]["step"]) == 1 and float(opt.norm) == math.inf
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        q = other.param_groups[0]["params"][0]
+        q.grad = torch.ones_like(q)
+        other.step()
+        assert other.skip_nonfinite and int(other.state[q]["step"]) == 2 and not torch.equal(q, kept)
