@@ -6,6 +6,7 @@
 // its gradient and two states and writes three of them back (22 bytes with 16-bit weights and 32-bit
 // states, 10 bytes with 8-bit states).
 #include <algorithm>
+#include <atomic>
 #include <math.h>
 #include <new>
 
@@ -157,10 +158,12 @@ __device__ __forceinline__ unsigned code_e4m3(float x, float inverse, unsigned r
   return (((b & 0x7fffffffu) + random20) >> 20) | ((b >> 24) & 0x80u);
 }
 
+constexpr unsigned kLeastV = 1u << 21;     // the code 1
+
 // v never becomes zero beside larger values: it is at least the format's smallest number (2^-32 of the
 // block's largest value), so an element is not divided by its eps alone because its neighbours are large.
 __device__ __forceinline__ unsigned code_e5m2(float x, float inverse, unsigned random21) {
-  const float y = fmaxf(__fmul_rn(__fmul_rn(x, inverse), 0x1p-112f), __uint_as_float(0x00200000u));
+  const float y = fmaxf(__fmul_rn(__fmul_rn(x, inverse), 0x1p-112f), __uint_as_float(kLeastV));
   return (__float_as_uint(y) + random21) >> 21;
 }
 
@@ -169,103 +172,150 @@ __device__ __forceinline__ float scale_of(unsigned largest, float factor) {
   return s >= FLT_MIN ? s : 0.0f;
 }
 
-__device__ __forceinline__ float2 widen_fp8x2(unsigned two, __nv_fp8_interpretation_t kind) {
-  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, kind)));
+// Two e4m3 / e5m2 codes, widened.  An e5m2 code is the upper half of a 16-bit float.
+__device__ __forceinline__ float2 widen_e4m3x2(unsigned two) {
+  return __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3)));
+}
+__device__ __forceinline__ float2 widen_e5m2x2(unsigned halves) { return __half22float2(*reinterpret_cast<const __half2*>(&halves)); }
+
+// max(|a|, |b|, |c|), NaN if one of them is
+__device__ __forceinline__ float max_abs3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float y;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
+
+// Top bytes of four words, lowest first.
+__device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
+}
+
+// The 32-bit form has 22 bytes of traffic per element to hide its arithmetic behind, this one 10: at HBM
+// speed an SM may spend about 49 instructions on an element.  So the arithmetic is in packed pairs,
+// root and reciprocal are the approximate ones (2 u each; they only reach the parameter), the codes are
+// formed in the top byte of a word, where shift and random bits are one addition, and one hash serves
+// a pair of elements.
 template <typename P, typename G, bool MASTER, int N>
 __global__ void __launch_bounds__(kOptThreads) adamw8_kernel(const __grid_constant__ OptBatch<N> b) {
   OptCoefs co;
   if (!opt_coefs(b.s, co)) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int i = 0;
+  const auto both = [](float x) { return make_float2(x, x); };
+  int i = -1;
+  unsigned key = 0;
   for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
-    i = opt_find<N>(b, c, i);
+    if (i < 0 || c >= b.first[i + 1]) {
+      i = opt_find<N>(b, c, max(i, 0));
+      key = opt_key(b.s.seed, co.t, b.t[i].index);
+    }
     const OptTensor& t = b.t[i];
     const long long e0 = (long long)(c - b.first[i]) * kOptChunk + warp * kOptBlock;
     if (e0 >= t.numel) continue;      // the same for the whole warp
     const bool vec = t.vec && e0 + kOptBlock <= t.numel;
     const long long blk = e0 / kOptBlock;
-    const unsigned key = opt_key(b.s.seed, co.t, t.index);
-    float p[8], g[8], m[8], v[8];
+    const unsigned unit_key = key + (unsigned)(e0 >> 33);
+    float p[8], g[8];
+    float2 m[4], v[4];
+    unsigned char* m8 = reinterpret_cast<unsigned char*>(t.exp_avg) + e0;
+    unsigned char* v8 = reinterpret_cast<unsigned char*>(t.exp_avg_sq) + e0;
+    if (vec) {
+      const uint2 cm = *reinterpret_cast<const uint2*>(m8 + lane * 8);
+      const uint2 cv = *reinterpret_cast<const uint2*>(v8 + lane * 8);
+      m[0] = widen_e4m3x2(cm.x & 0xffffu), m[1] = widen_e4m3x2(cm.x >> 16);
+      m[2] = widen_e4m3x2(cm.y & 0xffffu), m[3] = widen_e4m3x2(cm.y >> 16);
+      v[0] = widen_e5m2x2(__byte_perm(cv.x, 0, 0x1404)), v[1] = widen_e5m2x2(__byte_perm(cv.x, 0, 0x3424));
+      v[2] = widen_e5m2x2(__byte_perm(cv.y, 0, 0x1404)), v[3] = widen_e5m2x2(__byte_perm(cv.y, 0, 0x3424));
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int e = j * 64 + lane;
+        const unsigned has0 = e < t.numel - e0, has1 = e + 32 < t.numel - e0;
+        m[j] = widen_e4m3x2((has0 ? m8[e] : 0u) | (has1 ? m8[e + 32] : 0u) << 8);
+        v[j] = widen_e5m2x2((has0 ? v8[e] : 0u) << 8 | (has1 ? v8[e + 32] : 0u) << 24);
+      }
+    }
     if (MASTER)
       opt_load<float>(t.master, e0, t.numel, vec, lane, 32, p);
     else
       opt_load<P>(t.param, e0, t.numel, vec, lane, 32, p);
     opt_load<G>(t.grad, e0, t.numel, vec, lane, 32, g);
-    const float sm = t.exp_avg_scale[blk], sv = t.exp_avg_sq_scale[blk];
-    unsigned char* m8 = reinterpret_cast<unsigned char*>(t.exp_avg);
-    unsigned char* v8 = reinterpret_cast<unsigned char*>(t.exp_avg_sq);
-    if (vec) {
-      const uint2 cm = *reinterpret_cast<const uint2*>(m8 + e0 + lane * 8);
-      const uint2 cv = *reinterpret_cast<const uint2*>(v8 + e0 + lane * 8);
+    const float2 sm = both(t.exp_avg_scale[blk]), sv = both(t.exp_avg_sq_scale[blk]);
+    // Products that are added to something are multiply-adds with a -0 that the compiler cannot see: it
+    // would contract a packed product and a packed sum, which are to be rounded one by one.
+    const float2 zero = both(b.s.minus_zero);
+    float top_m = 0.0f, top_v = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; j += 2) {
-        const float2 a = widen_fp8x2((j < 4 ? cm.x : cm.y) >> (j & 2) * 8 & 0xffffu, __NV_E4M3);
-        const float2 q = widen_fp8x2((j < 4 ? cv.x : cv.y) >> (j & 2) * 8 & 0xffffu, __NV_E5M2);
-        m[j] = a.x, m[j + 1] = a.y, v[j] = q.x, v[j + 1] = q.y;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const long long e = e0 + j * 32 + lane;
-        m[j] = e < t.numel ? widen_fp8x2(m8[e], __NV_E4M3).x : 0.0f;
-        v[j] = e < t.numel ? widen_fp8x2(v8[e], __NV_E5M2).x : 0.0f;
-      }
-    }
-    unsigned top_m = 0, top_v = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      m[j] = __fmul_rn(m[j], sm);
-      v[j] = __fmul_rn(v[j], sv);
-      opt_moments(b.s, __fmul_rn(g[j], co.clip), m[j], v[j]);
-      p[j] = adamw_param(b.s, co, p[j], m[j], v[j]);
-      top_m = max(top_m, __float_as_uint(m[j]) & 0x7fffffffu);
-      top_v = max(top_v, __float_as_uint(v[j]) & 0x7fffffffu);
+    for (int j = 0; j < 4; j++) {
+      const float2 gj = mul2(make_float2(g[2 * j], g[2 * j + 1]), both(co.clip));
+      m[j] = add2(fma2(both(b.s.beta1), mul2(m[j], sm), zero), fma2(both(b.s.one_minus_beta1), gj, zero));
+      v[j] = add2(fma2(both(b.s.beta2), mul2(v[j], sv), zero), fma2(both(b.s.one_minus_beta2), mul2(gj, gj), zero));
+      const float2 d = fma2(make_float2(sqrt_approx(v[j].x), sqrt_approx(v[j].y)), both(co.root), both(b.s.eps));
+      const float2 q = mul2(m[j], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
+      const float2 pj = fma2(both(-co.rate), q, mul2(make_float2(p[2 * j], p[2 * j + 1]), both(co.decay)));
+      p[2 * j] = pj.x, p[2 * j + 1] = pj.y;
+      top_m = max_abs3(top_m, m[j].x, m[j].y);
+      top_v = max_abs3(top_v, v[j].x, v[j].y);
     }
     opt_store<P>(t.param, e0, t.numel, vec, lane, 32, p);
     if (MASTER) opt_store<float>(t.master, e0, t.numel, vec, lane, 32, p);
-    top_m = __reduce_max_sync(0xffffffffu, top_m);
-    top_v = __reduce_max_sync(0xffffffffu, top_v);
-    const bool odd_values = max(top_m, top_v) >= 0x7f800000u;
-    if (odd_values) {                 // infinities and NaN keep to their own elements: the scale is that of the others
-      top_m = top_v = 0;
+    unsigned largest_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
+    unsigned largest_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
+    const bool strange = max(largest_m, largest_v) >= 0x7f800000u;
+    if (strange) {                    // infinities and NaN keep to their own elements: the scale is that of the others
+      top_m = top_v = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const unsigned bm = __float_as_uint(m[j]) & 0x7fffffffu, bv = __float_as_uint(v[j]) & 0x7fffffffu;
-        if (bm < 0x7f800000u) top_m = max(top_m, bm);
-        if (bv < 0x7f800000u) top_v = max(top_v, bv);
+      for (int j = 0; j < 4; j++) {
+        if (!not_finite(m[j].x)) top_m = fmaxf(top_m, fabsf(m[j].x));
+        if (!not_finite(m[j].y)) top_m = fmaxf(top_m, fabsf(m[j].y));
+        if (!not_finite(v[j].x)) top_v = fmaxf(top_v, v[j].x);
+        if (!not_finite(v[j].y)) top_v = fmaxf(top_v, v[j].y);
       }
-      top_m = __reduce_max_sync(0xffffffffu, top_m);
-      top_v = __reduce_max_sync(0xffffffffu, top_v);
+      largest_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
+      largest_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
     }
-    const float new_sm = scale_of(top_m, kScaleM), new_sv = scale_of(top_v, kScaleV);
+    const float new_sm = scale_of(largest_m, kScaleM), new_sv = scale_of(largest_v, kScaleV);
     const float im = new_sm > 0.0f ? __frcp_rn(new_sm) : 0.0f, iv = new_sv > 0.0f ? __frcp_rn(new_sv) : 0.0f;
-    unsigned qm[8], qv[8];
+    if (vec && !strange) {
+      // element 2 j takes bits 12..31 of the pair's hash for m and 0..20 for v, element 2 j + 1 bits 0..19 and
+      // 11..31: as 24 bits under the top byte that is h >> 8 for two of them
+      const unsigned pair = ((unsigned)(e0 >> 1) | lane * 4);
+      unsigned qm[8], qv[8];
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      const long long e = vec ? e0 + lane * 8 + j : e0 + j * 32 + lane;
-      const unsigned h = opt_mix((unsigned)(e >> 1) ^ (key + (unsigned)(e >> 33)));
-      qm[j] = code_e4m3(m[j], im, e & 1 ? h & 0xfffffu : h >> 12);
-      qv[j] = code_e5m2(v[j], iv, e & 1 ? h >> 11 : h & 0x1fffffu);
-      if (odd_values) {
-        if ((__float_as_uint(m[j]) & 0x7fffffffu) >= 0x7f800000u) qm[j] = 0x7f;
-        if ((__float_as_uint(v[j]) & 0x7fffffffu) >= 0x7f800000u) qv[j] = 0x7f;
+      for (int j = 0; j < 4; j++) {
+        const unsigned h = opt_mix((pair | j) ^ unit_key);
+        const float2 ym = mul2(mul2(m[j], both(im)), both(0x1p-120f));
+        const float2 yv = mul2(mul2(v[j], both(iv)), both(0x1p-112f));
+        const unsigned m0 = __float_as_uint(ym.x), m1 = __float_as_uint(ym.y);
+        const unsigned v0 = __float_as_uint(fmaxf(yv.x, __uint_as_float(kLeastV))), v1 = __float_as_uint(fmaxf(yv.y, __uint_as_float(kLeastV)));
+        qm[2 * j] = ((m0 << 4) + (h >> 8)) | (m0 & 0x80000000u);
+        qm[2 * j + 1] = ((m1 << 4) + (h << 4 & 0xffffffu)) | (m1 & 0x80000000u);
+        qv[2 * j] = (v0 << 3) + (h << 3 & 0xffffffu);
+        qv[2 * j + 1] = (v1 << 3) + (h >> 8);
       }
-    }
-    if (vec) {
-      *reinterpret_cast<uint2*>(m8 + e0 + lane * 8) =
-          make_uint2(qm[0] | qm[1] << 8 | qm[2] << 16 | qm[3] << 24, qm[4] | qm[5] << 8 | qm[6] << 16 | qm[7] << 24);
-      *reinterpret_cast<uint2*>(v8 + e0 + lane * 8) =
-          make_uint2(qv[0] | qv[1] << 8 | qv[2] << 16 | qv[3] << 24, qv[4] | qv[5] << 8 | qv[6] << 16 | qv[7] << 24);
+      *reinterpret_cast<uint2*>(m8 + lane * 8) = make_uint2(top_bytes(qm[0], qm[1], qm[2], qm[3]), top_bytes(qm[4], qm[5], qm[6], qm[7]));
+      *reinterpret_cast<uint2*>(v8 + lane * 8) = make_uint2(top_bytes(qv[0], qv[1], qv[2], qv[3]), top_bytes(qv[4], qv[5], qv[6], qv[7]));
     } else {
 #pragma unroll
       for (int j = 0; j < 8; j++) {
-        const long long e = e0 + j * 32 + lane;
-        if (e < t.numel) {
-          m8[e] = (unsigned char)qm[j];
-          v8[e] = (unsigned char)qv[j];
-        }
+        const int e = vec ? lane * 8 + j : j * 32 + lane;
+        if (e >= t.numel - e0) continue;
+        const float mj = j & 1 ? m[j >> 1].y : m[j >> 1].x, vj = j & 1 ? v[j >> 1].y : v[j >> 1].x;
+        const unsigned h = opt_mix(((unsigned)(e0 >> 1) | e >> 1) ^ unit_key);
+        m8[e] = (unsigned char)(not_finite(mj) ? 0x7fu : code_e4m3(mj, im, e & 1 ? h & 0xfffffu : h >> 12));
+        v8[e] = (unsigned char)(not_finite(vj) ? 0x7fu : code_e5m2(vj, iv, e & 1 ? h >> 11 : h & 0x1fffffu));
       }
     }
     if (lane == 0) {
@@ -366,7 +416,7 @@ static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_
 
 constexpr int64_t kOptMaxTensors = 1 << 16;
 constexpr int64_t kOptMaxNumel = 1ll << 40;
-constexpr int kOptGrid = 148 * 8;       // CTAs of a launch at most; each takes every gridDim-th chunk
+constexpr int kOptSms = 148;
 constexpr int kSmallBatch = 16, kLargeBatch = 256;
 
 // A stretch of memory that a step reads or writes.
@@ -403,6 +453,7 @@ static OptScalars make_scalars(int64_t* step, double lr, const float* lr_device,
   s.one_minus_beta2 = (float)(1.0 - beta2);
   s.eps = (float)eps;
   s.max_norm = (float)max_norm;
+  s.minus_zero = -0.0f;
   s.seed = seed;
   s.advance = 0;
   return s;
@@ -481,9 +532,9 @@ static OptTensor make_tensor(const flexsae_optim_tensor& t, int64_t i, int state
   d.master = t.master;
   d.numel = t.numel;
   d.index = (int)i;
-  const size_t state_align = state_bits == 8 ? 8 : 16;
-  d.vec = aligned(t.param, 16) && aligned(t.grad, 16) && aligned(t.master, 16) && aligned(t.exp_avg, state_align) &&
-          aligned(t.exp_avg_sq, state_align);
+  const size_t state = state_bits == 8 ? 8 : 32;
+  d.vec = aligned(t.param, 8 * opt_size(t.param_dtype)) && aligned(t.grad, 8 * opt_size(t.grad_dtype)) && aligned(t.master, 32) &&
+          aligned(t.exp_avg, state) && aligned(t.exp_avg_sq, state);
   return d;
 }
 
@@ -493,6 +544,15 @@ constexpr int kOptKinds = 9;
 static int kind_of(const flexsae_optim_tensor& t) {
   if (t.param_dtype == FLEXSAE_F32) return 0;
   return 1 + (t.param_dtype == FLEXSAE_F16 ? 4 : 0) + (t.grad_dtype == FLEXSAE_F32 ? 2 : 0) + (t.master ? 1 : 0);
+}
+
+// CTAs of `threads` that the GPU holds at the same time: the grid of a launch whose CTAs take every
+// gridDim-th unit, so that all of them run from the start and finish together.
+template <typename K>
+static unsigned resident_ctas(K kernel, int threads) {
+  int n = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
+  return (unsigned)(n * kOptSms);
 }
 
 #define FLEXSAE_OPT_KINDS(kind, CALL)                         \
@@ -510,10 +570,14 @@ static int kind_of(const flexsae_optim_tensor& t) {
 
 template <int N>
 static cudaError_t launch_adamw(const OptBatch<N>& b, int kind, int state_bits, cudaStream_t st) {
-  const unsigned grid = std::max(1u, std::min(b.chunks, (unsigned)kOptGrid));
 #define CALL_ADAMW(P, G, M)                                                                       \
-  if (state_bits == 8) adamw8_kernel<P, G, M, N><<<grid, kOptThreads, 0, st>>>(b);                \
-  else adamw_kernel<P, G, M, N><<<grid, kOptThreads, 0, st>>>(b)
+  {                                                                                               \
+    const auto kernel = state_bits == 8 ? adamw8_kernel<P, G, M, N> : adamw_kernel<P, G, M, N>;   \
+    static const unsigned most[2] = {resident_ctas(adamw_kernel<P, G, M, N>, kOptThreads),        \
+                                     resident_ctas(adamw8_kernel<P, G, M, N>, kOptThreads)};      \
+    const unsigned grid = std::max(1u, std::min(b.chunks, most[state_bits == 8]));                \
+    kernel<<<grid, kOptThreads, 0, st>>>(b);                                                      \
+  }
   FLEXSAE_OPT_KINDS(kind, CALL_ADAMW)
 #undef CALL_ADAMW
   t_launches++;
@@ -574,9 +638,14 @@ static int adamw_impl(const flexsae_optim_tensor* t, int64_t n, int state_bits, 
 
 static cudaError_t launch_rows(const RowArgs& a, int kind, cudaStream_t st) {
   const int warps = (a.cols + kOptBlock - 1) / kOptBlock;
-  const int per_sm = std::max(1, std::min(32, 64 / warps));
-  const unsigned grid = (unsigned)std::max<long long>(1, std::min<long long>(a.rows, 148ll * per_sm));
-#define CALL_ROWS(P, G, M) adamw_unit_rows_kernel<P, G, M><<<grid, warps * 32, 0, st>>>(a)
+#define CALL_ROWS(P, G, M)                                                                        \
+  {                                                                                               \
+    static std::atomic<unsigned> most[33];                                                        \
+    unsigned m = most[warps].load(std::memory_order_relaxed);                                     \
+    if (!m) most[warps] = m = resident_ctas(adamw_unit_rows_kernel<P, G, M>, warps * 32);         \
+    const unsigned grid = (unsigned)std::min<long long>(a.rows, m);                               \
+    adamw_unit_rows_kernel<P, G, M><<<grid, warps * 32, 0, st>>>(a);                              \
+  }
   FLEXSAE_OPT_KINDS(kind, CALL_ROWS)
 #undef CALL_ROWS
   t_launches++;
@@ -635,7 +704,7 @@ int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, 
       b.grad[b.count] = grads_host[i];
       b.numel[b.count] = numel_host[i];
       b.dtype[b.count] = (unsigned char)dtypes_host[i];
-      b.vec[b.count] = aligned(grads_host[i], 16);
+      b.vec[b.count] = aligned(grads_host[i], 8 * opt_size(dtypes_host[i]));
       b.first[++b.count] = (unsigned)chunks;
     }
     b.chunks = (unsigned)chunks;
