@@ -9,6 +9,7 @@
 #include <atomic>
 #include <math.h>
 #include <new>
+#include <type_traits>
 
 #include "flexsae_optim.cuh"
 
@@ -16,7 +17,7 @@ namespace flexsae {
 
 // ---- gradient norm --------------------------------------------------------------------------------------
 constexpr int kNormUnits = 4;                               // units of 256 elements a warp takes at a time
-constexpr int kNormChunk = kOptChunk * kNormUnits;
+constexpr int kNormChunk = kOptThreads / 32 * kOptBlock * kNormUnits;
 constexpr int kNormGrid = 148 * 8;
 
 template <int N>
@@ -33,7 +34,8 @@ struct NormBatch {
 // Sum of eight squares.  The plain 32-bit sum is used where it neither overflowed nor lost terms to
 // underflow; otherwise the squares are formed in 64 bits, so that a norm is finite whenever the
 // result fits the output.
-__device__ __forceinline__ double sum_squares(const float* x) {
+__device__ __forceinline__ double sum_squares(const float2* pairs) {
+  const float* x = reinterpret_cast<const float*>(pairs);
   float s = 0.0f;
 #pragma unroll
   for (int j = 0; j < 8; j++) s = fmaf(x[j], x[j], s);
@@ -63,14 +65,14 @@ template <typename T>
 __device__ __forceinline__ double norm_chunk(const void* grad, long long e0, long long numel, bool aligned, int lane) {
   double acc = 0.0;
   if (aligned && e0 + kNormUnits * kOptBlock <= numel) {
-    float x[kNormUnits][8];
+    float2 x[kNormUnits][4];
 #pragma unroll
     for (int u = 0; u < kNormUnits; u++) opt_load<T>(grad, e0 + u * kOptBlock, numel, true, lane, 32, x[u]);
 #pragma unroll
     for (int u = 0; u < kNormUnits; u++) acc += sum_squares(x[u]);
   } else {
     for (int u = 0; u < kNormUnits; u++) {
-      float x[8];
+      float2 x[4];
       opt_load<T>(grad, e0 + u * kOptBlock, numel, false, lane, 32, x);
       acc += sum_squares(x);
     }
@@ -105,41 +107,127 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_finish_kernel(const dou
   if (threadIdx.x == 0) *out = (float)sqrt(acc);
 }
 
+constexpr int kAdamwThreads = 128, kAdamw8Threads = 256;
+
 // ---- AdamW, 32-bit states -----------------------------------------------------------------------------
-__device__ __forceinline__ float adamw_param(const OptScalars& s, const OptCoefs& c, float p, float m, float v) {
-  return p * c.decay - c.rate * (m / (sqrtf(v) * c.root + s.eps));
+__device__ __forceinline__ float sqrt_approx(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 
-template <typename P, typename G, bool MASTER, int N>
-__global__ void __launch_bounds__(kOptThreads) adamw_kernel(const __grid_constant__ OptBatch<N> b) {
-  OptCoefs co;
-  if (!opt_coefs(b.s, co)) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// The chunks of all tensors (a unit for every one of a CTA's warps) are dealt out to the CTAs in turn.  Step is told about
+//   full(first, end, stride)  its complete, aligned chunks of a tensor, which lie in one span of 2^31 elements;
+//                             answers the first one that it has not done (for this warp), from which on units go to
+//   part(unit)                which does any unit, for the whole warp.
+template <int N, typename Step>
+__device__ __forceinline__ void opt_walk(const OptBatch<N>& b, Step& step) {
+  constexpr int kChunk = Step::kThreads * 8;
+  constexpr unsigned kSpan = (1u << 31) / kChunk;
   int i = 0;
-  for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
+  for (unsigned c = blockIdx.x; c < b.chunks;) {
     i = opt_find<N>(b, c, i);
     const OptTensor& t = b.t[i];
-    const long long e0 = (long long)(c - b.first[i]) * kOptChunk + warp * kOptBlock;
-    if (e0 >= t.numel) continue;
-    const bool vec = t.vec && e0 + kOptBlock <= t.numel;
-    float p[8], g[8], m[8], v[8];
-    if (MASTER)
-      opt_load<float>(t.master, e0, t.numel, vec, lane, 32, p);
-    else
-      opt_load<P>(t.param, e0, t.numel, vec, lane, 32, p);
-    opt_load<G>(t.grad, e0, t.numel, vec, lane, 32, g);
-    opt_load<float>(t.exp_avg, e0, t.numel, vec, lane, 32, m);
-    opt_load<float>(t.exp_avg_sq, e0, t.numel, vec, lane, 32, v);
+    const unsigned first = b.first[i], last = b.first[i + 1];
+    step.tensor(t);
+    const unsigned whole = t.vec ? (unsigned)(t.numel / kChunk) : 0u;
+    unsigned rest = c - first;
+    while (rest < whole) {
+      const unsigned end = min(whole, (rest / kSpan + 1) * kSpan);
+      rest = step.full(rest, end, gridDim.x);
+      if (rest < end) break;
+    }
+    for (; rest < last - first; rest += gridDim.x) {
+      const unsigned u = rest * (Step::kThreads / 32) + (threadIdx.x >> 5);
+      if ((long long)u * kOptBlock < t.numel) step.part(u);
+    }
+    c += ((last - 1 - c) / gridDim.x + 1) * gridDim.x;
+  }
+}
+
+// One step of two elements, the same bits wherever it is taken: the moments, then the parameter.  Products that
+// are added to something are multiply-adds with a -0 that the compiler cannot see: it would contract a packed
+// product and a packed sum, which are to be rounded one by one (see opt_moments).  Root and reciprocal are
+// approximate, 2 u each: they only reach the parameter.
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+__device__ __forceinline__ void moments_pair(const OptScalars& s, float clip, float2 g, float2& m, float2& v) {
+  const float2 zero = both(s.minus_zero);
+  g = mul2(g, both(clip));
+  m = add2(fma2(both(s.beta1), m, zero), fma2(both(s.one_minus_beta1), g, zero));
+  v = add2(fma2(both(s.beta2), v, zero), fma2(both(s.one_minus_beta2), mul2(g, g), zero));
+}
+
+__device__ __forceinline__ float2 param_pair(const OptScalars& s, const OptCoefs& c, float2 p, float2 m, float2 v) {
+  const float2 d = fma2(make_float2(sqrt_approx(v.x), sqrt_approx(v.y)), both(c.root), both(s.eps));
+  return fma2(both(-c.rate), mul2(m, make_float2(rcp_approx(d.x), rcp_approx(d.y))), mul2(p, both(c.decay)));
+}
+
+// The approximate root takes subnormal second moments as zero: roots below 2^-63, which with b2 = 0.999 are
+// at most 2^-58 in the denominator and nothing beside an eps from here on.  Below it the step is taken with
+// IEEE root and division, one element at a time.
+constexpr float kLeastEps = 0x1p-33f;
+
+__device__ __forceinline__ void adamw_eight(const OptScalars& s, const OptCoefs& c, float2* p, const float2* g, float2* m, float2* v) {
+  if (s.eps >= kLeastEps) {
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      moments_pair(s, c.clip, g[j], m[j], v[j]);
+      p[j] = param_pair(s, c, p[j], m[j], v[j]);
+    }
+  } else {
+    float *ps = reinterpret_cast<float*>(p), *ms = reinterpret_cast<float*>(m), *vs = reinterpret_cast<float*>(v);
+    const float* gs = reinterpret_cast<const float*>(g);
 #pragma unroll
     for (int j = 0; j < 8; j++) {
-      opt_moments(b.s, __fmul_rn(g[j], co.clip), m[j], v[j]);
-      p[j] = adamw_param(b.s, co, p[j], m[j], v[j]);
+      opt_moments(s, __fmul_rn(gs[j], c.clip), ms[j], vs[j]);
+      ps[j] = ps[j] * c.decay - c.rate * (ms[j] / (sqrtf(vs[j]) * c.root + s.eps));
     }
-    opt_store<P>(t.param, e0, t.numel, vec, lane, 32, p);
-    if (MASTER) opt_store<float>(t.master, e0, t.numel, vec, lane, 32, p);
-    opt_store<float>(t.exp_avg, e0, t.numel, vec, lane, 32, m);
-    opt_store<float>(t.exp_avg_sq, e0, t.numel, vec, lane, 32, v);
   }
+}
+
+template <typename P, typename G, bool MASTER>
+struct AdamwStep {
+  static constexpr int kThreads = kAdamwThreads;
+  using W = typename std::conditional<MASTER, float, P>::type;      // type that holds the parameter's value
+  const OptScalars& s;
+  const OptCoefs& co;
+  const OptTensor* t;
+
+  __device__ __forceinline__ void tensor(const OptTensor& x) { t = &x; }
+
+  // Elements e0 + lane * 8 ... of a team of `lanes` threads, or every lanes-th of them.
+  __device__ __forceinline__ void unit(long long e0, bool vec, int lane, int lanes) const {
+    float2 p[4], g[4], m[4], v[4];
+    opt_load<W>(MASTER ? t->master : t->param, e0, t->numel, vec, lane, lanes, p);
+    opt_load<G>(t->grad, e0, t->numel, vec, lane, lanes, g);
+    opt_load<float>(t->exp_avg, e0, t->numel, vec, lane, lanes, m);
+    opt_load<float>(t->exp_avg_sq, e0, t->numel, vec, lane, lanes, v);
+    adamw_eight(s, co, p, g, m, v);
+    opt_store<P>(t->param, e0, t->numel, vec, lane, lanes, p);
+    if (MASTER) opt_store<float>(t->master, e0, t->numel, vec, lane, lanes, p);
+    opt_store<float>(t->exp_avg, e0, t->numel, vec, lane, lanes, m);
+    opt_store<float>(t->exp_avg_sq, e0, t->numel, vec, lane, lanes, v);
+  }
+
+  __device__ __forceinline__ unsigned full(unsigned c, unsigned end, unsigned stride) const {
+    for (; c < end; c += stride) unit((long long)c * (kThreads * 8), true, threadIdx.x, kThreads);
+    return c;
+  }
+  __device__ __forceinline__ void part(unsigned u) const { unit((long long)u * kOptBlock, false, threadIdx.x & 31, 32); }
+};
+
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kAdamwThreads, 4) adamw_kernel(const __grid_constant__ OptBatch<N> b) {
+  OptCoefs co;
+  if (!opt_coefs(b.s, co)) return;
+  AdamwStep<P, G, MASTER> step{b.s, co, nullptr};
+  opt_walk<N>(b, step);
   opt_advance(b.s, co.t);
 }
 
@@ -171,6 +259,7 @@ __device__ __forceinline__ float scale_of(unsigned largest, float factor) {
   const float s = __fmul_rn(__uint_as_float(largest), factor);
   return s >= FLT_MIN ? s : 0.0f;
 }
+__device__ __forceinline__ float inverse_of(float scale) { return scale > 0.0f ? __frcp_rn(scale) : 0.0f; }
 
 // Two e4m3 / e5m2 codes, widened.  An e5m2 code is the upper half of a 16-bit float.
 __device__ __forceinline__ float2 widen_e4m3x2(unsigned two) {
@@ -185,144 +274,196 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {
   return d;
 }
 
-__device__ __forceinline__ float sqrt_approx(float x) {
-  float y;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
-__device__ __forceinline__ bool not_finite(float x) { return !(fabsf(x) <= FLT_MAX); }
+__device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 
 // Top bytes of four words, lowest first.
 __device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
+  // The step, to the same bits as Adamw8Step, for a unit that is cut off, not aligned, or holds an infinity or NaN, which
+  // keep to their own elements: the scale is that of the others.  With an eps below kLeastEps, for which the
+  // approximate root is not good enough, all units come here.
+  template <typename P, typename G, bool MASTER>
+__device__ __forceinline__ void adamw8_part(const OptScalars& s, const OptCoefs& co, const OptTensor* t, unsigned key, unsigned u) {
+  using W = typename std::conditional<MASTER, float, P>::type;
+  const int lane = threadIdx.x & 31;
+    const long long e0 = (long long)u * kOptBlock;
+    const int n = (int)min((long long)kOptBlock, t->numel - e0);
+    unsigned char* m8 = reinterpret_cast<unsigned char*>(t->exp_avg) + e0;
+    unsigned char* v8 = reinterpret_cast<unsigned char*>(t->exp_avg_sq) + e0;
+    const float sm = t->exp_avg_scale[u], sv = t->exp_avg_sq_scale[u];
+    float2 p[4], g[4], m[4], v[4];
+    opt_load<W>(MASTER ? t->master : t->param, e0, t->numel, false, lane, 32, p);
+    opt_load<G>(t->grad, e0, t->numel, false, lane, 32, g);
+    float* ms = reinterpret_cast<float*>(m);
+    float* vs = reinterpret_cast<float*>(v);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int e = j * 32 + lane;
+      ms[j] = __fmul_rn(widen_e4m3x2(e < n ? m8[e] : 0u).x, sm);
+      vs[j] = __fmul_rn(widen_e5m2x2(e < n ? v8[e] << 8 : 0u).x, sv);
+    }
+    adamw_eight(s, co, p, g, m, v);
+    float top_m = 0.0f, top_v = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      if (finite(ms[j])) top_m = fmaxf(top_m, fabsf(ms[j]));
+      if (finite(vs[j])) top_v = fmaxf(top_v, vs[j]);
+    }
+    opt_store<P>(t->param, e0, t->numel, false, lane, 32, p);
+    if (MASTER) opt_store<float>(t->master, e0, t->numel, false, lane, 32, p);
+    const float new_sm = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_m)), kScaleM);
+    const float new_sv = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top_v)), kScaleV);
+    const float im = inverse_of(new_sm), iv = inverse_of(new_sv);
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const int e = j * 32 + lane;
+      if (e >= n) continue;
+      const unsigned h = opt_mix((u * (kOptBlock / 2) + (e >> 1)) ^ (key + (u >> 25)));
+      m8[e] = (unsigned char)(finite(ms[j]) ? code_e4m3(ms[j], im, e & 1 ? h & 0xfffffu : h >> 12) : 0x7fu);
+      v8[e] = (unsigned char)(finite(vs[j]) ? code_e5m2(vs[j], iv, e & 1 ? h >> 11 : h & 0x1fffffu) : 0x7fu);
+    }
+    if (lane == 0) {
+      t->exp_avg_scale[u] = new_sm;
+      t->exp_avg_sq_scale[u] = new_sv;
+    }
+  }
+
 // The 32-bit form has 22 bytes of traffic per element to hide its arithmetic behind, this one 10: at HBM
 // speed an SM may spend about 49 instructions on an element.  So the arithmetic is in packed pairs,
 // root and reciprocal are the approximate ones (2 u each; they only reach the parameter), the codes are
-// formed in the top byte of a word, where shift and random bits are one addition, and one hash serves
-// a pair of elements.
-template <typename P, typename G, bool MASTER, int N>
-__global__ void __launch_bounds__(kOptThreads) adamw8_kernel(const __grid_constant__ OptBatch<N> b) {
-  OptCoefs co;
-  if (!opt_coefs(b.s, co)) return;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const auto both = [](float x) { return make_float2(x, x); };
-  int i = -1;
-  unsigned key = 0;
-  for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
-    if (i < 0 || c >= b.first[i + 1]) {
-      i = opt_find<N>(b, c, max(i, 0));
-      key = opt_key(b.s.seed, co.t, b.t[i].index);
+// formed in the top byte of a word, where shift and random bits are one addition, one hash serves a
+// pair of elements, and a warp's next unit is on its way while it works on one.
+template <typename P, typename G, bool MASTER>
+struct Adamw8Step {
+  static constexpr int kThreads = kAdamw8Threads;
+  using W = typename std::conditional<MASTER, float, P>::type;      // type that holds the parameter's value
+  struct Raw {
+    Raw8<W> p;
+    Raw8<G> g;
+    Raw8<unsigned char> m, v;
+    float sm, sv;
+  };
+  const OptScalars& s;
+  const OptCoefs& co;
+  const OptTensor* t;
+  unsigned key;
+
+  __device__ __forceinline__ void tensor(const OptTensor& x) {
+    t = &x;
+    key = opt_key(s.seed, co.t, x.index);
+  }
+
+  // Where this thread's eight elements of a chunk begin, and its warp's scales.
+  struct Place {
+    const W* w;
+    P* p;
+    const G* g;
+    unsigned char *m, *v;
+    float *sm, *sv;
+    unsigned pair, high;      // half the element's index: low 32 bits, and the key with the high ones
+  };
+
+  // `e` elements on from the place: 32 bits are enough, and one instruction makes an address.
+  __device__ __forceinline__ static void fetch(const Place& at, unsigned e, Raw& r) {
+    r.p.load(at.w + e);
+    r.g.load(at.g + e);
+    r.m.load(at.m + e);
+    r.v.load(at.v + e);
+    r.sm = at.sm[e / kOptBlock];
+    r.sv = at.sv[e / kOptBlock];
+  }
+
+  __device__ __forceinline__ unsigned full(unsigned c, unsigned end, unsigned stride) const {
+    const size_t e0 = (size_t)c * (kThreads * 8) + threadIdx.x * 8;
+    Place at;
+    at.p = reinterpret_cast<P*>(t->param) + e0;
+    at.w = MASTER ? reinterpret_cast<const W*>(t->master + e0) : reinterpret_cast<const W*>(at.p);
+    at.g = reinterpret_cast<const G*>(t->grad) + e0;
+    at.m = reinterpret_cast<unsigned char*>(t->exp_avg) + e0;
+    at.v = reinterpret_cast<unsigned char*>(t->exp_avg_sq) + e0;
+    at.sm = t->exp_avg_scale + e0 / kOptBlock;
+    at.sv = t->exp_avg_sq_scale + e0 / kOptBlock;
+    at.pair = (unsigned)(e0 / 2);
+    at.high = key + (unsigned)(e0 >> 33);
+    Raw next;
+    fetch(at, 0, next);
+    unsigned e = 0;
+    for (; c < end; c += stride, e += stride * (kThreads * 8)) {
+      const Raw now = next;
+      if (c + stride < end) fetch(at, e + stride * (kThreads * 8), next);
+      if (!unit(now, at, e)) break;
     }
-    const OptTensor& t = b.t[i];
-    const long long e0 = (long long)(c - b.first[i]) * kOptChunk + warp * kOptBlock;
-    if (e0 >= t.numel) continue;      // the same for the whole warp
-    const bool vec = t.vec && e0 + kOptBlock <= t.numel;
-    const long long blk = e0 / kOptBlock;
-    const unsigned unit_key = key + (unsigned)(e0 >> 33);
-    float p[8], g[8];
-    float2 m[4], v[4];
-    unsigned char* m8 = reinterpret_cast<unsigned char*>(t.exp_avg) + e0;
-    unsigned char* v8 = reinterpret_cast<unsigned char*>(t.exp_avg_sq) + e0;
-    if (vec) {
-      const uint2 cm = *reinterpret_cast<const uint2*>(m8 + lane * 8);
-      const uint2 cv = *reinterpret_cast<const uint2*>(v8 + lane * 8);
-      m[0] = widen_e4m3x2(cm.x & 0xffffu), m[1] = widen_e4m3x2(cm.x >> 16);
-      m[2] = widen_e4m3x2(cm.y & 0xffffu), m[3] = widen_e4m3x2(cm.y >> 16);
-      v[0] = widen_e5m2x2(__byte_perm(cv.x, 0, 0x1404)), v[1] = widen_e5m2x2(__byte_perm(cv.x, 0, 0x3424));
-      v[2] = widen_e5m2x2(__byte_perm(cv.y, 0, 0x1404)), v[3] = widen_e5m2x2(__byte_perm(cv.y, 0, 0x3424));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const int e = j * 64 + lane;
-        const unsigned has0 = e < t.numel - e0, has1 = e + 32 < t.numel - e0;
-        m[j] = widen_e4m3x2((has0 ? m8[e] : 0u) | (has1 ? m8[e + 32] : 0u) << 8);
-        v[j] = widen_e5m2x2((has0 ? v8[e] : 0u) << 8 | (has1 ? v8[e + 32] : 0u) << 24);
-      }
-    }
-    if (MASTER)
-      opt_load<float>(t.master, e0, t.numel, vec, lane, 32, p);
-    else
-      opt_load<P>(t.param, e0, t.numel, vec, lane, 32, p);
-    opt_load<G>(t.grad, e0, t.numel, vec, lane, 32, g);
-    const float2 sm = both(t.exp_avg_scale[blk]), sv = both(t.exp_avg_sq_scale[blk]);
-    // Products that are added to something are multiply-adds with a -0 that the compiler cannot see: it
-    // would contract a packed product and a packed sum, which are to be rounded one by one.
-    const float2 zero = both(b.s.minus_zero);
+    return c;
+  }
+
+  // False: the unit holds an infinity or NaN, and nothing was written.
+  __device__ __forceinline__ bool unit(const Raw& r, const Place& at, unsigned e) const {
+    float2 p[4], g[4], m[4], v[4];
+    m[0] = widen_e4m3x2(r.m.w.x & 0xffffu), m[1] = widen_e4m3x2(r.m.w.x >> 16);
+    m[2] = widen_e4m3x2(r.m.w.y & 0xffffu), m[3] = widen_e4m3x2(r.m.w.y >> 16);
+    v[0] = widen_e5m2x2(__byte_perm(r.v.w.x, 0, 0x1404)), v[1] = widen_e5m2x2(__byte_perm(r.v.w.x, 0, 0x3424));
+    v[2] = widen_e5m2x2(__byte_perm(r.v.w.y, 0, 0x1404)), v[3] = widen_e5m2x2(__byte_perm(r.v.w.y, 0, 0x3424));
+    r.g.pairs(g);
     float top_m = 0.0f, top_v = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; j++) {
-      const float2 gj = mul2(make_float2(g[2 * j], g[2 * j + 1]), both(co.clip));
-      m[j] = add2(fma2(both(b.s.beta1), mul2(m[j], sm), zero), fma2(both(b.s.one_minus_beta1), gj, zero));
-      v[j] = add2(fma2(both(b.s.beta2), mul2(v[j], sv), zero), fma2(both(b.s.one_minus_beta2), mul2(gj, gj), zero));
-      const float2 d = fma2(make_float2(sqrt_approx(v[j].x), sqrt_approx(v[j].y)), both(co.root), both(b.s.eps));
-      const float2 q = mul2(m[j], make_float2(rcp_approx(d.x), rcp_approx(d.y)));
-      const float2 pj = fma2(both(-co.rate), q, mul2(make_float2(p[2 * j], p[2 * j + 1]), both(co.decay)));
-      p[2 * j] = pj.x, p[2 * j + 1] = pj.y;
+      m[j] = mul2(m[j], both(r.sm));
+      v[j] = mul2(v[j], both(r.sv));
+      moments_pair(s, co.clip, g[j], m[j], v[j]);
       top_m = max_abs3(top_m, m[j].x, m[j].y);
       top_v = max_abs3(top_v, v[j].x, v[j].y);
     }
-    opt_store<P>(t.param, e0, t.numel, vec, lane, 32, p);
-    if (MASTER) opt_store<float>(t.master, e0, t.numel, vec, lane, 32, p);
-    unsigned largest_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
-    unsigned largest_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
-    const bool strange = max(largest_m, largest_v) >= 0x7f800000u;
-    if (strange) {                    // infinities and NaN keep to their own elements: the scale is that of the others
-      top_m = top_v = 0.0f;
+    const unsigned largest_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
+    const unsigned largest_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
+    if (max(largest_m, largest_v) >= 0x7f800000u) return false;
+    r.p.pairs(p);
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        if (!not_finite(m[j].x)) top_m = fmaxf(top_m, fabsf(m[j].x));
-        if (!not_finite(m[j].y)) top_m = fmaxf(top_m, fabsf(m[j].y));
-        if (!not_finite(v[j].x)) top_v = fmaxf(top_v, v[j].x);
-        if (!not_finite(v[j].y)) top_v = fmaxf(top_v, v[j].y);
-      }
-      largest_m = __reduce_max_sync(0xffffffffu, __float_as_uint(top_m));
-      largest_v = __reduce_max_sync(0xffffffffu, __float_as_uint(top_v));
-    }
+    for (int j = 0; j < 4; j++) p[j] = param_pair(s, co, p[j], m[j], v[j]);
+    opt_store8<P>(at.p + e, p);
+    if (MASTER) opt_store8<float>(reinterpret_cast<float*>(const_cast<W*>(at.w)) + e, p);
     const float new_sm = scale_of(largest_m, kScaleM), new_sv = scale_of(largest_v, kScaleV);
-    const float im = new_sm > 0.0f ? __frcp_rn(new_sm) : 0.0f, iv = new_sv > 0.0f ? __frcp_rn(new_sv) : 0.0f;
-    if (vec && !strange) {
-      // element 2 j takes bits 12..31 of the pair's hash for m and 0..20 for v, element 2 j + 1 bits 0..19 and
-      // 11..31: as 24 bits under the top byte that is h >> 8 for two of them
-      const unsigned pair = ((unsigned)(e0 >> 1) | lane * 4);
-      unsigned qm[8], qv[8];
+    const float2 im = both(inverse_of(new_sm)), iv = both(inverse_of(new_sv));
+    // element 2 j takes bits 12..31 of the pair's hash for m and 0..20 for v, element 2 j + 1 bits 0..19 and
+    // 11..31: as 24 bits under the top byte that is h >> 8 for two of them.  The first step of the hash is
+    // the same for the four pairs of a lane but for their last two bits.
+    const unsigned x = (at.pair + e / 2) ^ at.high;
+    unsigned qm[8], qv[8];
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const unsigned h = opt_mix((pair | j) ^ unit_key);
-        const float2 ym = mul2(mul2(m[j], both(im)), both(0x1p-120f));
-        const float2 yv = mul2(mul2(v[j], both(iv)), both(0x1p-112f));
-        const unsigned m0 = __float_as_uint(ym.x), m1 = __float_as_uint(ym.y);
-        const unsigned v0 = __float_as_uint(fmaxf(yv.x, __uint_as_float(kLeastV))), v1 = __float_as_uint(fmaxf(yv.y, __uint_as_float(kLeastV)));
-        qm[2 * j] = ((m0 << 4) + (h >> 8)) | (m0 & 0x80000000u);
-        qm[2 * j + 1] = ((m1 << 4) + (h << 4 & 0xffffffu)) | (m1 & 0x80000000u);
-        qv[2 * j] = (v0 << 3) + (h << 3 & 0xffffffu);
-        qv[2 * j + 1] = (v1 << 3) + (h >> 8);
-      }
-      *reinterpret_cast<uint2*>(m8 + lane * 8) = make_uint2(top_bytes(qm[0], qm[1], qm[2], qm[3]), top_bytes(qm[4], qm[5], qm[6], qm[7]));
-      *reinterpret_cast<uint2*>(v8 + lane * 8) = make_uint2(top_bytes(qv[0], qv[1], qv[2], qv[3]), top_bytes(qv[4], qv[5], qv[6], qv[7]));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; j++) {
-        const int e = vec ? lane * 8 + j : j * 32 + lane;
-        if (e >= t.numel - e0) continue;
-        const float mj = j & 1 ? m[j >> 1].y : m[j >> 1].x, vj = j & 1 ? v[j >> 1].y : v[j >> 1].x;
-        const unsigned h = opt_mix(((unsigned)(e0 >> 1) | e >> 1) ^ unit_key);
-        m8[e] = (unsigned char)(not_finite(mj) ? 0x7fu : code_e4m3(mj, im, e & 1 ? h & 0xfffffu : h >> 12));
-        v8[e] = (unsigned char)(not_finite(vj) ? 0x7fu : code_e5m2(vj, iv, e & 1 ? h >> 11 : h & 0x1fffffu));
-      }
+    for (int j = 0; j < 4; j++) {
+      const unsigned h = opt_mix_rest((x ^ x >> 16) ^ j);
+      const float2 ym = mul2(mul2(m[j], im), both(0x1p-120f));
+      const float2 yv = mul2(mul2(v[j], iv), both(0x1p-112f));
+      const unsigned m0 = __float_as_uint(ym.x), m1 = __float_as_uint(ym.y);
+      const unsigned v0 = __float_as_uint(fmaxf(yv.x, __uint_as_float(kLeastV))), v1 = __float_as_uint(fmaxf(yv.y, __uint_as_float(kLeastV)));
+      qm[2 * j] = ((m0 << 4) + (h >> 8)) | (m0 & 0x80000000u);
+      qm[2 * j + 1] = ((m1 << 4) + (h << 4 & 0xffffffu)) | (m1 & 0x80000000u);
+      qv[2 * j] = (v0 << 3) + (h << 3 & 0xffffffu);
+      qv[2 * j + 1] = (v1 << 3) + (h >> 8);
     }
-    if (lane == 0) {
-      t.exp_avg_scale[blk] = new_sm;
-      t.exp_avg_sq_scale[blk] = new_sv;
+    Raw8<unsigned char> cm, cv;
+    cm.w = make_uint2(top_bytes(qm[0], qm[1], qm[2], qm[3]), top_bytes(qm[4], qm[5], qm[6], qm[7]));
+    cv.w = make_uint2(top_bytes(qv[0], qv[1], qv[2], qv[3]), top_bytes(qv[4], qv[5], qv[6], qv[7]));
+    cm.store(at.m + e);
+    cv.store(at.v + e);
+    if (threadIdx.x % 32 == 0) {
+      at.sm[e / kOptBlock] = new_sm;
+      at.sv[e / kOptBlock] = new_sv;
     }
+    return true;
   }
+
+  __device__ __forceinline__ void part(unsigned u) const { adamw8_part<P, G, MASTER>(s, co, t, key, u); }
+};
+
+template <typename P, typename G, bool MASTER, int N>
+__global__ void __launch_bounds__(kAdamw8Threads, sizeof(P) == 4 || sizeof(G) == 4 || MASTER ? 2 : 3) adamw8_kernel(const __grid_constant__ OptBatch<N> b) {
+  OptCoefs co;
+  if (!opt_coefs(b.s, co)) return;
+  Adamw8Step<P, G, MASTER> step{b.s, co, nullptr, 0};
+  opt_walk<N>(b, step);
   opt_advance(b.s, co.t);
 }
 
@@ -361,24 +502,25 @@ template <typename P, typename G, bool MASTER>
 __global__ void __launch_bounds__(1024) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
   OptCoefs co;
   if (!opt_coefs(a.s, co)) return;
+  using W = typename std::conditional<MASTER, float, P>::type;
+  OptCoefs unclipped = co;      // the gradient is clipped before the projection
+  unclipped.clip = 1.0f;
   __shared__ float2 part[2][32];
   const int warps = blockDim.x >> 5, lanes = blockDim.x;
   const OptTensor& t = a.t;
   for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
     const long long e0 = r * a.cols, end = e0 + a.cols;
     const bool vec = t.vec && (int)threadIdx.x * 8 < a.cols;      // the last lanes of a row may have nothing
-    float p[8], g[8], m[8], v[8];
+    float2 p2[4], g2[4], m2[4], v2[4];
+    float *p = reinterpret_cast<float*>(p2), *g = reinterpret_cast<float*>(g2);
     if (t.vec && !vec) {
 #pragma unroll
-      for (int j = 0; j < 8; j++) p[j] = g[j] = m[j] = v[j] = 0.0f;
+      for (int j = 0; j < 4; j++) p2[j] = g2[j] = m2[j] = v2[j] = make_float2(0.0f, 0.0f);
     } else {
-      if (MASTER)
-        opt_load<float>(t.master, e0, end, vec, threadIdx.x, lanes, p);
-      else
-        opt_load<P>(t.param, e0, end, vec, threadIdx.x, lanes, p);
-      opt_load<G>(t.grad, e0, end, vec, threadIdx.x, lanes, g);
-      opt_load<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m);
-      opt_load<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v);
+      opt_load<W>(MASTER ? t.master : t.param, e0, end, vec, threadIdx.x, lanes, p2);
+      opt_load<G>(t.grad, e0, end, vec, threadIdx.x, lanes, g2);
+      opt_load<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m2);
+      opt_load<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v2);
     }
     float gp = 0.0f, pp = 0.0f;
 #pragma unroll
@@ -391,20 +533,19 @@ __global__ void __launch_bounds__(1024) adamw_unit_rows_kernel(const __grid_cons
     const float along = dots.y > 0.0f ? dots.x / dots.y : 0.0f;
     float len = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-      opt_moments(a.s, g[j] - along * p[j], m[j], v[j]);
-      p[j] = adamw_param(a.s, co, p[j], m[j], v[j]);
-      len = fmaf(p[j], p[j], len);
-    }
+    for (int j = 0; j < 8; j++) g[j] -= along * p[j];
+    adamw_eight(a.s, unclipped, p2, g2, m2, v2);
+#pragma unroll
+    for (int j = 0; j < 8; j++) len = fmaf(p[j], p[j], len);
     len = cta_sum2(len, 0.0f, part[1], warps).x;
     const float scale = len > 0.0f ? 1.0f / sqrtf(len) : 1.0f;      // a row of zeros stays one
 #pragma unroll
     for (int j = 0; j < 8; j++) p[j] *= scale;
     if (t.vec && !vec) continue;
-    opt_store<P>(t.param, e0, end, vec, threadIdx.x, lanes, p);
-    if (MASTER) opt_store<float>(t.master, e0, end, vec, threadIdx.x, lanes, p);
-    opt_store<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m);
-    opt_store<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v);
+    opt_store<P>(t.param, e0, end, vec, threadIdx.x, lanes, p2);
+    if (MASTER) opt_store<float>(t.master, e0, end, vec, threadIdx.x, lanes, p2);
+    opt_store<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m2);
+    opt_store<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v2);
   }
   opt_advance(a.s, co.t);
 }
@@ -415,7 +556,8 @@ static bool opt_dtype(int dt) { return dt == FLEXSAE_F32 || dt == FLEXSAE_BF16 |
 static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
 
 constexpr int64_t kOptMaxTensors = 1 << 16;
-constexpr int64_t kOptMaxNumel = 1ll << 40;
+constexpr int64_t kOptMaxNumel = 1ll << 38;
+constexpr unsigned long long kOptMaxChunks = 1ull << 30;
 constexpr int kOptSms = 148;
 constexpr int kSmallBatch = 16, kLargeBatch = 256;
 
@@ -466,7 +608,7 @@ static int check_tensor(const flexsae_optim_tensor& t, int64_t i, int state_bits
   if (t.grad_dtype != t.param_dtype && t.grad_dtype != FLEXSAE_F32)
     return fail(FLEXSAE_EINVAL, "tensor %lld: the gradient's type (code %d) must be the parameter's or fp32", at, t.grad_dtype);
   if (t.master && t.param_dtype == FLEXSAE_F32) return fail(FLEXSAE_EINVAL, "tensor %lld: a master copy goes with 16-bit parameters only", at);
-  if (t.numel < 0 || t.numel > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^40]", at, (long long)t.numel);
+  if (t.numel < 0 || t.numel > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^38]", at, (long long)t.numel);
   *used = 0;
   if (t.numel == 0) return 0;
   if (rows) {
@@ -549,10 +691,10 @@ static int kind_of(const flexsae_optim_tensor& t) {
 // CTAs of `threads` that the GPU holds at the same time: the grid of a launch whose CTAs take every
 // gridDim-th unit, so that all of them run from the start and finish together.
 template <typename K>
-static unsigned resident_ctas(K kernel, int threads) {
+static unsigned resident_ctas(K kernel, int threads, int most = 32) {
   int n = 0;
   if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
-  return (unsigned)(n * kOptSms);
+  return (unsigned)(std::min(n, most) * kOptSms);
 }
 
 #define FLEXSAE_OPT_KINDS(kind, CALL)                         \
@@ -568,15 +710,22 @@ static unsigned resident_ctas(K kernel, int threads) {
     default: CALL(__half, float, true); break;                \
   }
 
+// What the loads of one SM have under way at most in the 32-bit step, which sets how many CTAs it is given.
+// More costs HBM throughput: 302 M bf16 parameters take 1.10 / 1.03 / 1.08 ms with 3 / 4 / 5 CTAs of 12 KB
+// each, 268 M fp32 parameters 1.25 / 1.12 / 1.18 ms with 2 / 3 / 4 of 16 KB.
+constexpr int kBytesInFlight = 48 * 1024;
+
 template <int N>
 static cudaError_t launch_adamw(const OptBatch<N>& b, int kind, int state_bits, cudaStream_t st) {
-#define CALL_ADAMW(P, G, M)                                                                       \
-  {                                                                                               \
-    const auto kernel = state_bits == 8 ? adamw8_kernel<P, G, M, N> : adamw_kernel<P, G, M, N>;   \
-    static const unsigned most[2] = {resident_ctas(adamw_kernel<P, G, M, N>, kOptThreads),        \
-                                     resident_ctas(adamw8_kernel<P, G, M, N>, kOptThreads)};      \
-    const unsigned grid = std::max(1u, std::min(b.chunks, most[state_bits == 8]));                \
-    kernel<<<grid, kOptThreads, 0, st>>>(b);                                                      \
+  const unsigned ctas = std::max(1u, b.chunks);
+#define CALL_ADAMW(P, G, M)                                                                             \
+  if (state_bits == 8) {                                                                                \
+    static const unsigned most = resident_ctas(adamw8_kernel<P, G, M, N>, kAdamw8Threads);              \
+    adamw8_kernel<P, G, M, N><<<std::min(ctas, most), kAdamw8Threads, 0, st>>>(b);                      \
+  } else {                                                                                              \
+    constexpr int bytes = 8 * ((M ? 4 : sizeof(P)) + sizeof(G) + 8);                                    \
+    static const unsigned most = resident_ctas(adamw_kernel<P, G, M, N>, kAdamwThreads, kBytesInFlight / (kAdamwThreads * bytes)); \
+    adamw_kernel<P, G, M, N><<<std::min(ctas, most), kAdamwThreads, 0, st>>>(b);                        \
   }
   FLEXSAE_OPT_KINDS(kind, CALL_ADAMW)
 #undef CALL_ADAMW
@@ -596,9 +745,11 @@ static cudaError_t run_kind(const flexsae_optim_tensor* t, const int* ids, int n
     unsigned long long chunks = 0;
     b.first[0] = 0;
     while (k < n && b.count < N) {
-      const OptTensor d = make_tensor(t[ids[k]], ids[k], state_bits);
-      const unsigned long long c = ((unsigned long long)d.numel + kOptChunk - 1) / kOptChunk;
-      if (b.count && chunks + c > 0x7fffffffull) break;
+      OptTensor d = make_tensor(t[ids[k]], ids[k], state_bits);
+      if (state_bits == 8 && s.eps < kLeastEps) d.vec = 0;
+      const unsigned long long chunk = 8 * (state_bits == 8 ? kAdamw8Threads : kAdamwThreads);
+      const unsigned long long c = ((unsigned long long)d.numel + chunk - 1) / chunk;
+      if (b.count && chunks + c > kOptMaxChunks) break;
       chunks += c;
       b.t[b.count++] = d;
       b.first[b.count] = (unsigned)chunks;
@@ -683,7 +834,7 @@ int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, 
   if (workspace_bytes < need) return fail(FLEXSAE_EWORKSPACE, "gradient norm workspace too small: %zu < %zu bytes", workspace_bytes, need);
   for (int64_t i = 0; i < n; i++) {
     if (!opt_dtype(dtypes_host[i])) return fail(FLEXSAE_EINVAL, "tensor %lld: unknown dtype code %d", (long long)i, dtypes_host[i]);
-    if (numel_host[i] < 0 || numel_host[i] > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^40]", (long long)i, (long long)numel_host[i]);
+    if (numel_host[i] < 0 || numel_host[i] > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^38]", (long long)i, (long long)numel_host[i]);
     if (numel_host[i] > 0 && !grads_host[i]) return fail(FLEXSAE_EINVAL, "tensor %lld: null pointer argument", (long long)i);
     if (!aligned(grads_host[i], opt_size(dtypes_host[i]))) return fail(FLEXSAE_EINVAL, "tensor %lld: a pointer is not aligned to its elements", (long long)i);
   }

@@ -147,7 +147,7 @@ def _entry(n=1, rows=False, bits=32, lr=1e-3, lr_dev=None, betas=(0.9, 0.999), e
     (dict(count=-1), "tensors"), (dict(count=1 << 20), "tensors"), (dict(table=False), "null"),
     (dict(param=0), "null"), (dict(grad=0), "null"), (dict(m=0), "null"), (dict(v=0), "null"),
     (dict(bits=8, ms=0), "scales"), (dict(bits=8, vs=0), "scales"),
-    (dict(numel=-1), "numel"), (dict(numel=1 << 41), "numel"), (dict(pdt=7), "dtype"), (dict(pdt=nv.BF16, gdt=nv.F16), "gradient"),
+    (dict(numel=-1), "numel"), (dict(numel=1 << 39), "numel"), (dict(pdt=7), "dtype"), (dict(pdt=nv.BF16, gdt=nv.F16), "gradient"),
     (dict(pdt=nv.F32, gdt=nv.BF16), "gradient"), (dict(master=7 << 20), "master"),
     (dict(param=(1 << 20) + 2), "aligned"), (dict(pdt=nv.BF16, grad=(2 << 20) + 2), "aligned"), (dict(pdt=nv.BF16, gdt=nv.BF16, param=(1 << 20) + 1), "aligned"),
     (dict(pdt=nv.BF16, master=(7 << 20) + 2), "aligned"), (dict(bits=8, ms=(5 << 20) + 1), "aligned"),
