@@ -9,6 +9,7 @@ loaded, e.g. ``wait_limit_ms=60000`` for a job whose ranks may drift far apart).
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from typing import Optional
 
@@ -63,6 +64,7 @@ SIGNATURES = {
 }
 
 _lib: Optional[ctypes.CDLL] = None
+_binding = None
 
 
 class FlexSaeNativeError(RuntimeError):
@@ -101,6 +103,32 @@ def load() -> ctypes.CDLL:
         name, _, value = item.partition("=")
         check(lib.flexsae_set_option(name.strip().encode(), int(value)), f"FLEXSAE_OPTIONS: {item}")
     return lib
+
+
+def binding():
+    """The compiled binding of the optimizer entry points (building it first if its source is newer), bound to the
+    library that ``load`` loaded."""
+    global _binding
+    if _binding is not None:
+        return _binding
+    lib = load()
+    path = _build.binding_path()
+    if os.environ.get("FLEXSAE_NO_BUILD", "0") != "1":
+        try:
+            path = _build.build_binding()
+        except RuntimeError:
+            if not os.path.exists(path):
+                raise
+    if not os.path.exists(path):
+        raise FlexSaeNativeError(f"{path} is missing: build it with `python -m flexsae_b200.build` (needs g++ and torch's headers)")
+    spec = importlib.util.spec_from_file_location("flexsae_binding", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    module.init(FlexSaeNativeError, *(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+        "flexsae_adamw_step", "flexsae_adamw_unit_rows_step", "flexsae_grad_norm", "flexsae_grad_norm_workspace_bytes",
+        "flexsae_last_error", "flexsae_last_launch_count")))
+    _binding = module
+    return module
 
 
 def check(rc: int, what: str) -> None:

@@ -1,4 +1,5 @@
-"""Builds the CUDA library in-tree: ``flexsae_b200/_lib/libflexsae_b200.so`` for sm_100a.
+"""Builds the CUDA library in-tree: ``flexsae_b200/_lib/libflexsae_b200.so`` for sm_100a, and the Python
+binding of its optimizer entry points (``csrc/host``, plain C++ against torch) beside it.
 
 nvcc cross-compiles without a GPU, so this runs on a CPU-only machine; the shared object then
 travels with the source tree.  ``python -m flexsae_b200.build`` rebuilds when a source is newer
@@ -86,5 +87,44 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
     return out
 
 
+def binding_path() -> str:
+    """The binding is tied to the interpreter and the torch it was compiled for; both are in its name."""
+    import torch
+
+    return os.path.join(LIB_DIR, f"flexsae_binding.torch-{torch.__version__}.cp{sys.version_info[0]}{sys.version_info[1]}.so")
+
+
+def build_binding(force: bool = False) -> str:
+    """Compiles ``csrc/host/flexsae_binding.cpp`` against the installed torch and returns the library's path."""
+    out = binding_path()
+    src = os.path.join(CSRC, "host", "flexsae_binding.cpp")
+    header = os.path.join(INCLUDE, "flexsae_b200.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return out
+    import sysconfig
+
+    import torch
+
+    cxx = shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: the Python binding cannot be built on this machine")
+    os.makedirs(LIB_DIR, exist_ok=True)
+    root = os.path.dirname(torch.__file__)
+    cuda = os.environ.get("CUDA_HOME", "/usr/local/cuda")
+    include = [os.path.join(root, "include"), sysconfig.get_paths()["include"], os.path.join(cuda, "include")]
+    tmp = f"{out}.{os.getpid()}.tmp"
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}"]
+    cmd += [f"-I{d}" for d in include] + [src, "-o", tmp, "-L" + os.path.join(root, "lib")]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+    res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        if os.path.exists(tmp):
+            os.remove(tmp)
+        raise RuntimeError("g++ failed:\n" + res.stdout[-4000:])
+    os.replace(tmp, out)
+    return out
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv, trace="--trace" in sys.argv))
+    print(build_binding(force="--force" in sys.argv))

@@ -19,8 +19,6 @@ so replicas that step on the same gradients stay equal.
 """
 from __future__ import annotations
 
-import ctypes
-import math
 from typing import Dict, Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
@@ -33,7 +31,7 @@ BLOCK = 256
 #: types of the 8-bit states: first moment, second moment
 STATE8_DTYPES = (torch.float8_e4m3fn, torch.float8_e5m2)
 
-_WORDS = 10          # 64-bit words of flexsae_optim_tensor
+_ADAMW, _ADAMW8, _UNIT_ROWS = 0, 1, 2      # kinds of step in the binding
 _Tensors = Sequence[torch.Tensor]
 _Masters = Sequence[Optional[torch.Tensor]]
 
@@ -43,180 +41,18 @@ def state8_blocks(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
-def _dense(t: torch.Tensor) -> bool:
-    """True if the elements fill a stretch of memory without gaps, each once (in any order of dimensions)."""
-    if t.is_contiguous():
-        return True
-    expected = 1
-    for stride, size in sorted((st, n) for st, n in zip(t.stride(), t.shape) if n != 1):
-        if stride != expected:
-            return t.numel() == 0
-        expected *= size
-    return True
-
-
-def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
-    return all(n == 1 or x == y for x, y, n in zip(a.stride(), b.stride(), a.shape))
-
-
-def _check_word(name: str, t: torch.Tensor, dtype: torch.dtype, dev: torch.device) -> int:
-    if not isinstance(t, torch.Tensor) or t.numel() != 1:
-        raise ValueError(f"{name} must be a tensor of one element")
-    if t.dtype != dtype:
-        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.device != dev:
-        raise RuntimeError(f"{name} is on {t.device}, the parameters are on {dev}")
-    return t.data_ptr()
-
-
-def _check_list(name: str, ts: Optional[_Tensors], params: _Tensors, dtype: torch.dtype, dev: torch.device) -> None:
-    if len(ts) != len(params):
-        raise ValueError(f"{len(ts)} tensors in {name}, {len(params)} parameters")
-    for t, p in zip(ts, params):
-        if t.dtype != dtype:
-            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"a tensor in {name} is on {t.device}, the parameters are on {dev}")
-        if t.shape != p.shape or not _same_layout(t, p):
-            raise ValueError(f"a tensor in {name} has shape {tuple(t.shape)} and strides {t.stride()}, "
-                             f"its parameter {tuple(p.shape)} and {p.stride()}")
-
-
-def _check_scales(name: str, ts: _Tensors, params: _Tensors, dev: torch.device) -> None:
-    if len(ts) != len(params):
-        raise ValueError(f"{len(ts)} tensors in {name}, {len(params)} parameters")
-    for t, p in zip(ts, params):
-        if t.dtype != torch.float32:
-            raise TypeError(f"{name} must be float32, got {t.dtype}")
-        if t.device != dev:
-            raise RuntimeError(f"a tensor in {name} is on {t.device}, the parameters are on {dev}")
-        if t.shape != (state8_blocks(p.numel()),) or not t.is_contiguous():
-            raise ValueError(f"{name} of {p.numel()} elements is contiguous float32 [{state8_blocks(p.numel())}], "
-                             f"got {tuple(t.shape)}")
-
-
-def _check_params(params: _Tensors, grads: _Tensors, rows: bool) -> Tuple[torch.device, List[torch.Tensor]]:
-    """Checks parameters and gradients; returns the device and the gradients in their parameters' layout."""
-    if len(grads) != len(params):
-        raise ValueError(f"{len(grads)} gradients, {len(params)} parameters")
-    dev, got = params[0].device, []
-    if dev.type != "cuda":
-        raise RuntimeError("flexsae_b200.optim needs CUDA tensors: there is no CPU path")
-    for p, g in zip(params, grads):
-        if p.dtype not in nv.DTYPE_CODES:
-            raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
-        if g.layout != torch.strided:
-            raise TypeError(f"gradients must be dense tensors, got {g.layout}")
-        if g.dtype != p.dtype and g.dtype != torch.float32:
-            raise TypeError(f"the gradient of a {p.dtype} parameter must have its type or float32, got {g.dtype}")
-        if p.device != dev or g.device != dev:
-            raise RuntimeError(f"parameters and gradients must be on one device, got {p.device} and {g.device} beside {dev}")
-        if g.shape != p.shape:
-            raise ValueError(f"a gradient has shape {tuple(g.shape)}, its parameter {tuple(p.shape)}")
-        if not _dense(p):
-            raise ValueError(f"a parameter of shape {tuple(p.shape)} with strides {p.stride()} does not fill its memory")
-        if rows and (p.dim() != 2 or not p.is_contiguous()):
-            raise ValueError(f"unit rows need a contiguous [F, D] parameter, got {tuple(p.shape)} with strides {p.stride()}")
-        if not _same_layout(g, p):
-            g = torch.empty_like(p, dtype=g.dtype).copy_(g)
-        got.append(g)
-    return dev, got
-
-
-def _step(entry: str, params: _Tensors, grads: _Tensors, states: Sequence[Optional[_Tensors]], step: torch.Tensor, lr, betas, eps,
-          weight_decay, masters, norm, max_norm, rows: bool = False, bits: int = 32, seed: int = 0) -> None:
-    lib = nv.load()
-    params = [p.detach() for p in params]
-    if not params:
-        raise ValueError("no parameters")
-    dev, grads = _check_params(params, grads, rows)
-    exp_avgs, scales, exp_avg_sqs, sq_scales = states
-    kinds = STATE8_DTYPES if bits == 8 else (torch.float32, torch.float32)
-    _check_list("exp_avgs", exp_avgs, params, kinds[0], dev)
-    _check_list("exp_avg_sqs", exp_avg_sqs, params, kinds[1], dev)
-    if bits == 8:
-        _check_scales("exp_avg_scales", scales, params, dev)
-        _check_scales("exp_avg_sq_scales", sq_scales, params, dev)
-    if masters is not None:
-        if len(masters) != len(params):
-            raise ValueError(f"{len(masters)} masters, {len(params)} parameters")
-        held = [(t, p) for t, p in zip(masters, params) if t is not None]
-        if any(p.dtype == torch.float32 for _, p in held):
-            raise ValueError("masters go with 16-bit parameters only")
-        _check_list("masters", [t for t, _ in held], [p for _, p in held], torch.float32, dev)
-    step_ptr = _check_word("step", step, torch.int64, dev)
-    lr_ptr = None
-    if isinstance(lr, torch.Tensor):
-        lr, lr_ptr = 0.0, _check_word("lr", lr, torch.float32, dev)
-    if not (math.isfinite(lr) and lr >= 0):
-        raise ValueError(f"lr must be a finite number >= 0, got {lr}")
-    if not all(0 <= b < 1 for b in betas):
-        raise ValueError(f"betas must be in [0, 1), got {betas}")
-    if not (math.isfinite(eps) and eps >= 2.0 ** -126):
-        raise ValueError(f"eps must be a normal float32 number > 0, got {eps}")
-    if not (math.isfinite(weight_decay) and weight_decay >= 0):
-        raise ValueError(f"weight_decay must be a finite number >= 0, got {weight_decay}")
-    if max_norm is not None and (norm is None or not max_norm > 0):
-        raise ValueError("max_norm must be positive and goes with norm")
-    norm_ptr = None if norm is None else _check_word("norm", norm, torch.float32, dev)
-    if not 0 <= seed < 2 ** 32:
-        raise ValueError(f"seed must be in [0, 2**32), got {seed}")
-    n = len(params)
-    zeros = [0] * n
-    columns = (
-        [p.data_ptr() for p in params], [g.data_ptr() for g in grads],
-        [t.data_ptr() for t in exp_avgs], [t.data_ptr() for t in exp_avg_sqs],
-        [t.data_ptr() for t in scales] if bits == 8 else zeros, [t.data_ptr() for t in sq_scales] if bits == 8 else zeros,
-        [0 if t is None else t.data_ptr() for t in masters] if masters is not None else zeros,
-        [p.numel() for p in params], [p.shape[-1] for p in params] if rows else zeros,
-        [nv.DTYPE_CODES[p.dtype] | nv.DTYPE_CODES[g.dtype] << 32 for p, g in zip(params, grads)])
-    table = (ctypes.c_int64 * (_WORDS * n))()
-    for k, column in enumerate(columns):
-        table[k::_WORDS] = column
-    tail = [step_ptr, float(lr), lr_ptr, float(betas[0]), float(betas[1]), float(eps), float(weight_decay), norm_ptr,
-            math.inf if max_norm is None else float(max_norm)]
-    with torch.cuda.device(dev):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if rows:
-            rc = lib.flexsae_adamw_unit_rows_step(table, n, *tail, stream)
-        else:
-            rc = lib.flexsae_adamw_step(table, n, bits, *tail, seed, stream)
-    nv.check(rc, entry)
-    _losses.launch_count += lib.flexsae_last_launch_count()
-    written = [*params, *exp_avgs, *exp_avg_sqs, *(t for t in masters or () if t is not None)]
-    torch.autograd.graph.increment_version(written)      # what autograd saved of them is out of date now
+def _step(kind: int, params, grads, exp_avgs, scales, exp_avg_sqs, sq_scales, masters, step, lr, betas, eps, weight_decay, norm,
+          max_norm, seed=0) -> None:
+    _losses.launch_count += nv.binding().step(kind, params, grads, exp_avgs, scales, exp_avg_sqs, sq_scales, masters, step, lr,
+                                              tuple(betas), eps, weight_decay, norm, max_norm, seed)
 
 
 def grad_norm(grads: _Tensors) -> torch.Tensor:
     """``sqrt(sum of squares)`` over all tensors of a list (float32, bfloat16 or float16, mixed) as a
     0-dim float32 tensor: the ``norm`` of the step functions.  The squares are added in 64 bits in a
     fixed order: the result is reproducible, and finite whenever float32 can hold it."""
-    grads = list(grads)
-    if not grads:
-        raise ValueError("no gradients")
-    dev = grads[0].device
-    if dev.type != "cuda":
-        raise RuntimeError("flexsae_b200.optim needs CUDA tensors: there is no CPU path")
-    for i, g in enumerate(grads):
-        if g.layout != torch.strided:
-            raise TypeError(f"gradients must be dense tensors, got {g.layout}")
-        if g.dtype not in nv.DTYPE_CODES:
-            raise TypeError(f"gradients must be float32, bfloat16 or float16, got {g.dtype}")
-        if g.device != dev:
-            raise RuntimeError(f"gradients must be on one device, got {g.device} beside {dev}")
-        if not _dense(g):
-            grads[i] = g.contiguous()
-    lib = nv.load()
-    n = len(grads)
-    with torch.cuda.device(dev):
-        norm = torch.empty((), dtype=torch.float32, device=dev)
-        ws = torch.empty(lib.flexsae_grad_norm_workspace_bytes(n), dtype=torch.uint8, device=dev)
-        rc = lib.flexsae_grad_norm((ctypes.c_void_p * n)(*[g.data_ptr() for g in grads]),
-                                   (ctypes.c_int64 * n)(*[g.numel() for g in grads]),
-                                   (ctypes.c_int32 * n)(*[nv.DTYPE_CODES[g.dtype] for g in grads]), n, norm.data_ptr(),
-                                   ws.data_ptr(), ws.numel(), torch.cuda.current_stream(dev).cuda_stream)
-    nv.check(rc, "flexsae_grad_norm")
-    _losses.launch_count += lib.flexsae_last_launch_count()
+    norm, launches = nv.binding().grad_norm(grads)
+    _losses.launch_count += launches
     return norm
 
 
@@ -236,8 +72,7 @@ def adamw_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sq
     device (which a captured graph follows).  ``norm``: the norm of all gradients, from ``grad_norm``;
     with it c = min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves everything as it
     was.  A tensor given twice, or tensors that overlap, are refused."""
-    _step("flexsae_adamw_step", params, grads, (exp_avgs, None, exp_avg_sqs, None), step, lr, betas, eps, weight_decay, masters,
-          norm, max_norm)
+    _step(_ADAMW, params, grads, exp_avgs, None, exp_avg_sqs, None, masters, step, lr, betas, eps, weight_decay, norm, max_norm)
 
 
 def adamw8_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_scales: _Tensors, exp_avg_sqs: _Tensors,
@@ -253,8 +88,8 @@ def adamw8_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_s
     step changes by a thousandth).  The random bits are a function of (seed, t, position in the list,
     element).  A second moment is stored as at least 2^-16 of its scale.  An infinity or a NaN
     stays with its own element."""
-    _step("flexsae_adamw_step", params, grads, (exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales), step, lr, betas, eps,
-          weight_decay, masters, norm, max_norm, bits=8, seed=seed)
+    _step(_ADAMW8, params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, masters, step, lr, betas, eps,
+          weight_decay, norm, max_norm, seed)
 
 
 def adamw_unit_rows_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sqs: _Tensors, step: torch.Tensor, *,
@@ -264,8 +99,7 @@ def adamw_unit_rows_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, 
     """``adamw_step`` for decoders [F, D] (contiguous, D up to 8192) whose rows are kept at unit length: the
     gradient's component along its row is taken out first (g -= (g.w / w.w) w), and after the step
     the row is divided by its length.  A row of zeros stays one."""
-    _step("flexsae_adamw_unit_rows_step", params, grads, (exp_avgs, None, exp_avg_sqs, None), step, lr, betas, eps, weight_decay,
-          masters, norm, max_norm, rows=True)
+    _step(_UNIT_ROWS, params, grads, exp_avgs, None, exp_avg_sqs, None, masters, step, lr, betas, eps, weight_decay, norm, max_norm)
 
 
 class AdamW(torch.optim.Optimizer):
