@@ -51,7 +51,7 @@ SIGNATURES = {
     "flexsae_sort_by_decoder_row": (_c_int, [_c_vp, _c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp]),
     "flexsae_index_skew_workspace_bytes": (_c_sz, [_c_i64]),
     "flexsae_index_skew": (_c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_sz, _c_vp, _c_vp]),
-    "flexsae_grad_norm_workspace_bytes": (_c_sz, [_c_i64]),
+    "flexsae_grad_norm_workspace_bytes": (_c_int, [_c_i64, _c_i64, _c_vp]),
     "flexsae_grad_norm": (_c_int, [_c_vp] * 3 + [_c_i64] + [_c_vp] * 2 + [_c_sz, _c_vp]),
     "flexsae_adamw_step": (_c_int, [_c_vp, _c_i64, _c_int, _c_vp, _c_dbl, _c_vp] + [_c_dbl] * 4
                            + [_c_vp, _c_dbl, ctypes.c_uint32, _c_vp]),

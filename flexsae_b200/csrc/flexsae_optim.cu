@@ -5,6 +5,8 @@
 // Every operator is one pass over its data, bound by HBM: per parameter the step reads the parameter,
 // its gradient and two states and writes three of them back (22 bytes with 16-bit weights and 32-bit
 // states, 10 bytes with 8-bit states).
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <atomic>
 #include <math.h>
@@ -17,8 +19,10 @@ namespace flexsae {
 
 // ---- gradient norm --------------------------------------------------------------------------------------
 constexpr int kNormUnits = 4;                               // units of 256 elements a warp takes at a time
-constexpr int kNormChunk = kOptThreads / 32 * kOptBlock * kNormUnits;
 constexpr int kNormGrid = 148 * 8;
+constexpr int kNormCluster = 8, kNormClusterThreads = 512;
+constexpr int64_t kNormSmall = 1 << 19;                     // elements of a list for which one cluster is enough: four rounds
+constexpr int kSmallBatch = 16, kLargeBatch = 256;          // tensors of one launch
 
 template <int N>
 struct NormBatch {
@@ -50,14 +54,15 @@ __device__ __forceinline__ double sum_squares(const float2* pairs) {
   return d;
 }
 
+template <int THREADS>
 __device__ __forceinline__ double block_sum(double v) {
-  __shared__ double part[kOptThreads / 32];
+  __shared__ double part[THREADS / 32];
 #pragma unroll
   for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
   __syncthreads();
   v = 0.0;
-  for (int i = 0; i < kOptThreads / 32; i++) v += part[i];
+  for (int i = 0; i < THREADS / 32; i++) v += part[i];
   return v;
 }
 
@@ -80,14 +85,15 @@ __device__ __forceinline__ double norm_chunk(const void* grad, long long e0, lon
   return acc;
 }
 
-template <int N>
-__global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_constant__ NormBatch<N> b) {
+// Sum of this thread's share; a CTA takes every gridDim-th chunk of THREADS / 32 warps.
+template <int N, int THREADS>
+__device__ __forceinline__ double norm_share(const NormBatch<N>& b) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   double acc = 0.0;
   int i = 0;
   for (unsigned c = blockIdx.x; c < b.chunks; c += gridDim.x) {
     while (c >= b.first[i + 1]) i++;
-    const long long e0 = (long long)(c - b.first[i]) * kNormChunk + warp * (kNormUnits * kOptBlock);
+    const long long e0 = ((long long)(c - b.first[i]) * (THREADS / 32) + warp) * (kNormUnits * kOptBlock);
     if (e0 >= b.numel[i]) continue;
     if (b.dtype[i] == FLEXSAE_F32)
       acc += norm_chunk<float>(b.grad[i], e0, b.numel[i], b.vec[i], lane);
@@ -96,15 +102,39 @@ __global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_con
     else
       acc += norm_chunk<__half>(b.grad[i], e0, b.numel[i], b.vec[i], lane);
   }
-  acc = block_sum(acc);
-  if (threadIdx.x == 0) b.partial[blockIdx.x] = acc;
+  return acc;
+}
+
+template <int N>
+__global__ void __launch_bounds__(kOptThreads) grad_norm_kernel(const __grid_constant__ NormBatch<N> b) {
+  const double sum = block_sum<kOptThreads>(norm_share<N, kOptThreads>(b));
+  if (threadIdx.x == 0) b.partial[blockIdx.x] = sum;
 }
 
 __global__ void __launch_bounds__(kOptThreads) grad_norm_finish_kernel(const double* partial, int n, float* out) {
   double acc = 0.0;
   for (int i = threadIdx.x; i < n; i += kOptThreads) acc += partial[i];
-  acc = block_sum(acc);
+  acc = block_sum<kOptThreads>(acc);
   if (threadIdx.x == 0) *out = (float)sqrt(acc);
+}
+
+// Small lists in one launch without a workspace: the CTAs of one cluster leave their sums in the shared memory
+// of its first one.  A toy model of 66 k gradients, whose norm is all latency, takes 5.6 instead of 8.6 us.
+__global__ void __cluster_dims__(kNormCluster, 1, 1) __launch_bounds__(kNormClusterThreads)
+    grad_norm_small_kernel(const __grid_constant__ NormBatch<kSmallBatch> b, float* out) {
+  namespace cg = cooperative_groups;
+  __shared__ double sums[kNormCluster];
+  const cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();                                 // a CTA's shared memory may be written once it runs
+  const double sum = block_sum<kNormClusterThreads>(norm_share<kSmallBatch, kNormClusterThreads>(b));
+  cluster.barrier_wait();
+  if (threadIdx.x == 0) cluster.map_shared_rank(sums, 0)[cluster.block_rank()] = sum;
+  cluster.sync();
+  if (cluster.block_rank() == 0 && threadIdx.x == 0) {
+    double total = 0.0;
+    for (int i = 0; i < kNormCluster; i++) total += sums[i];
+    *out = (float)sqrt(total);
+  }
 }
 
 constexpr int kAdamwThreads = 128, kAdamw8Threads = 256;
@@ -496,31 +526,37 @@ __device__ __forceinline__ float2 cta_sum2(float a, float b, float2* part, int w
   return make_float2(a, b);
 }
 
-// One CTA per row at a time, eight elements per thread, so the row stays in registers between the
-// projection, the step and the division by its length.
-template <typename P, typename G, bool MASTER>
-__global__ void __launch_bounds__(1024) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
+// A team of warps per row at a time, eight elements per thread, so the row stays in registers between the
+// projection, the step and the division by its length.  The team is the CTA, or one of its warps where a warp is
+// enough for a row (rows of up to 256 elements; those need no barrier).
+// MOST: threads of a CTA at most.  Rows of up to 2304 elements (288 threads) are better off with four CTAs on an SM than
+// with the registers of three (65536 rows of 2304 bf16: 541 and 556 us); a fifth would spill (767 us).
+template <typename P, typename G, bool MASTER, int MOST>
+__global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
+  using W = typename std::conditional<MASTER, float, P>::type;
+  __shared__ float2 part[2][32];
+  const bool one_warp = a.cols <= kOptBlock;
+  const int teams = one_warp ? blockDim.x >> 5 : 1, lanes = one_warp ? 32 : blockDim.x, warps = lanes >> 5;
+  const int lane = one_warp ? threadIdx.x & 31 : threadIdx.x;
+  const OptTensor& t = a.t;
   OptCoefs co;
   if (!opt_coefs(a.s, co)) return;
-  using W = typename std::conditional<MASTER, float, P>::type;
-  OptCoefs unclipped = co;      // the gradient is clipped before the projection
+  OptCoefs unclipped = co;                            // the gradient is clipped before the projection
   unclipped.clip = 1.0f;
-  __shared__ float2 part[2][32];
-  const int warps = blockDim.x >> 5, lanes = blockDim.x;
-  const OptTensor& t = a.t;
-  for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+  const long long stride = (long long)gridDim.x * teams;
+  for (long long r = (long long)blockIdx.x * teams + (one_warp ? threadIdx.x >> 5 : 0); r < a.rows; r += stride) {
     const long long e0 = r * a.cols, end = e0 + a.cols;
-    const bool vec = t.vec && (int)threadIdx.x * 8 < a.cols;      // the last lanes of a row may have nothing
+    const bool vec = t.vec && lane * 8 < a.cols;      // the last lanes of an aligned row may have nothing
     float2 p2[4], g2[4], m2[4], v2[4];
     float *p = reinterpret_cast<float*>(p2), *g = reinterpret_cast<float*>(g2);
     if (t.vec && !vec) {
 #pragma unroll
       for (int j = 0; j < 4; j++) p2[j] = g2[j] = m2[j] = v2[j] = make_float2(0.0f, 0.0f);
     } else {
-      opt_load<W>(MASTER ? t.master : t.param, e0, end, vec, threadIdx.x, lanes, p2);
-      opt_load<G>(t.grad, e0, end, vec, threadIdx.x, lanes, g2);
-      opt_load<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m2);
-      opt_load<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v2);
+      opt_load<W>(MASTER ? t.master : t.param, e0, end, vec, lane, lanes, p2);
+      opt_load<G>(t.grad, e0, end, vec, lane, lanes, g2);
+      opt_load<float>(t.exp_avg, e0, end, vec, lane, lanes, m2);
+      opt_load<float>(t.exp_avg_sq, e0, end, vec, lane, lanes, v2);
     }
     float gp = 0.0f, pp = 0.0f;
 #pragma unroll
@@ -542,10 +578,10 @@ __global__ void __launch_bounds__(1024) adamw_unit_rows_kernel(const __grid_cons
 #pragma unroll
     for (int j = 0; j < 8; j++) p[j] *= scale;
     if (t.vec && !vec) continue;
-    opt_store<P>(t.param, e0, end, vec, threadIdx.x, lanes, p2);
-    if (MASTER) opt_store<float>(t.master, e0, end, vec, threadIdx.x, lanes, p2);
-    opt_store<float>(t.exp_avg, e0, end, vec, threadIdx.x, lanes, m2);
-    opt_store<float>(t.exp_avg_sq, e0, end, vec, threadIdx.x, lanes, v2);
+    opt_store<P>(t.param, e0, end, vec, lane, lanes, p2);
+    if (MASTER) opt_store<float>(t.master, e0, end, vec, lane, lanes, p2);
+    opt_store<float>(t.exp_avg, e0, end, vec, lane, lanes, m2);
+    opt_store<float>(t.exp_avg_sq, e0, end, vec, lane, lanes, v2);
   }
   opt_advance(a.s, co.t);
 }
@@ -559,7 +595,6 @@ constexpr int64_t kOptMaxTensors = 1 << 16;
 constexpr int64_t kOptMaxNumel = 1ll << 38;
 constexpr unsigned long long kOptMaxChunks = 1ull << 30;
 constexpr int kOptSms = 148;
-constexpr int kSmallBatch = 16, kLargeBatch = 256;
 
 // A stretch of memory that a step reads or writes.
 struct Stretch {
@@ -787,15 +822,19 @@ static int adamw_impl(const flexsae_optim_tensor* t, int64_t n, int state_bits, 
   return 0;
 }
 
+constexpr int kRowTeams = 4;      // warps of a CTA where each has a row of its own
+
 static cudaError_t launch_rows(const RowArgs& a, int kind, cudaStream_t st) {
-  const int warps = (a.cols + kOptBlock - 1) / kOptBlock;
-#define CALL_ROWS(P, G, M)                                                                        \
-  {                                                                                               \
-    static std::atomic<unsigned> most[33];                                                        \
-    unsigned m = most[warps].load(std::memory_order_relaxed);                                     \
-    if (!m) most[warps] = m = resident_ctas(adamw_unit_rows_kernel<P, G, M>, warps * 32);         \
-    const unsigned grid = (unsigned)std::min<long long>(a.rows, m);                               \
-    adamw_unit_rows_kernel<P, G, M><<<grid, warps * 32, 0, st>>>(a);                              \
+  const int row_warps = (a.cols + kOptBlock - 1) / kOptBlock;
+  const int teams = row_warps == 1 ? kRowTeams : 1, warps = row_warps * teams;
+  const long long ctas = (a.rows + teams - 1) / teams;
+#define CALL_ROWS(P, G, M)                                                                                    \
+  {                                                                                                           \
+    const auto kernel = warps <= 9 ? adamw_unit_rows_kernel<P, G, M, 288> : adamw_unit_rows_kernel<P, G, M, 1024>; \
+    static std::atomic<unsigned> most[33];                                                                    \
+    unsigned m = most[warps].load(std::memory_order_relaxed);                                                 \
+    if (!m) most[warps] = m = resident_ctas(kernel, warps * 32);                                              \
+    kernel<<<(unsigned)std::min<long long>(ctas, m), warps * 32, 0, st>>>(a);                                 \
   }
   FLEXSAE_OPT_KINDS(kind, CALL_ROWS)
 #undef CALL_ROWS
@@ -816,41 +855,42 @@ using namespace flexsae;
 
 extern "C" {
 
-size_t flexsae_grad_norm_workspace_bytes(int64_t n) {
-  if (n < 0 || n > kOptMaxTensors) {
-    fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
-    return 0;
-  }
-  return (size_t)((n + kLargeBatch - 1) / kLargeBatch + 1) * kNormGrid * sizeof(double);
+int flexsae_grad_norm_workspace_bytes(int64_t n, int64_t elements, size_t* bytes) {
+  if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
+  if (elements < 0 || !bytes) return fail(FLEXSAE_EINVAL, "%lld elements, or null pointer", (long long)elements);
+  *bytes = n <= kSmallBatch && elements <= kNormSmall ? 0 : (size_t)((n + kLargeBatch - 1) / kLargeBatch + 1) * kNormGrid * sizeof(double);
+  return 0;
 }
 
 int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, const int32_t* dtypes_host, int64_t n,
                       float* norm_out, void* workspace, size_t workspace_bytes, void* stream) {
   t_launches = 0;
   if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
-  if (!norm_out || !workspace || (n > 0 && (!grads_host || !numel_host || !dtypes_host))) return fail(FLEXSAE_EINVAL, "null pointer argument");
-  if (!aligned(workspace, 8)) return fail(FLEXSAE_EINVAL, "workspace must be 8-byte aligned");
-  const size_t need = flexsae_grad_norm_workspace_bytes(n);
-  if (workspace_bytes < need) return fail(FLEXSAE_EWORKSPACE, "gradient norm workspace too small: %zu < %zu bytes", workspace_bytes, need);
+  if (!norm_out || (n > 0 && (!grads_host || !numel_host || !dtypes_host))) return fail(FLEXSAE_EINVAL, "null pointer argument");
+  if (!aligned(norm_out, 4)) return fail(FLEXSAE_EINVAL, "norm_out must be 4-byte aligned");
+  int64_t elements = 0;
   for (int64_t i = 0; i < n; i++) {
     if (!opt_dtype(dtypes_host[i])) return fail(FLEXSAE_EINVAL, "tensor %lld: unknown dtype code %d", (long long)i, dtypes_host[i]);
     if (numel_host[i] < 0 || numel_host[i] > kOptMaxNumel) return fail(FLEXSAE_EINVAL, "tensor %lld: numel %lld outside [0, 2^38]", (long long)i, (long long)numel_host[i]);
     if (numel_host[i] > 0 && !grads_host[i]) return fail(FLEXSAE_EINVAL, "tensor %lld: null pointer argument", (long long)i);
     if (!aligned(grads_host[i], opt_size(dtypes_host[i]))) return fail(FLEXSAE_EINVAL, "tensor %lld: a pointer is not aligned to its elements", (long long)i);
+    elements += numel_host[i];
   }
+  size_t need = 0;
+  if (int rc = flexsae_grad_norm_workspace_bytes(n, elements, &need)) return rc;
+  if (need && (!workspace || !aligned(workspace, 8))) return fail(FLEXSAE_EINVAL, "workspace must be given, 8-byte aligned");
+  if (workspace_bytes < need) return fail(FLEXSAE_EWORKSPACE, "gradient norm workspace too small: %zu < %zu bytes", workspace_bytes, need);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-  double* partial = reinterpret_cast<double*>(workspace);
-  int parts = 0;
-  cudaError_t e = cudaSuccess;
   int64_t i = 0;
-  const auto gather = [&](auto& b, int most) {      // the next tensors, as many as fit
+  // The next tensors, as many as fit, in chunks of `chunk` elements.
+  const auto gather = [&](auto& b, int most, unsigned long long chunk) {
     unsigned long long chunks = 0;
     b.count = 0;
     b.first[0] = 0;
     for (; i < n && b.count < most; i++) {
-      const unsigned long long c = ((unsigned long long)numel_host[i] + kNormChunk - 1) / kNormChunk;
+      const unsigned long long c = ((unsigned long long)numel_host[i] + chunk - 1) / chunk;
       if (c == 0) continue;
-      if (b.count && chunks + c > 0x7fffffffull) break;
+      if (b.count && chunks + c > kOptMaxChunks) break;
       chunks += c;
       b.grad[b.count] = grads_host[i];
       b.numel[b.count] = numel_host[i];
@@ -859,25 +899,40 @@ int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, 
       b.first[++b.count] = (unsigned)chunks;
     }
     b.chunks = (unsigned)chunks;
-    b.partial = partial + parts;
-    if (!b.count) return;
-    const unsigned grid = std::min(b.chunks, (unsigned)kNormGrid);
-    e = launch_norm(b, grid, st);
-    parts += (int)grid;
+    b.partial = nullptr;
   };
-  while (i < n && e == cudaSuccess) {
-    if (n <= kSmallBatch) {
-      NormBatch<kSmallBatch> b;
-      gather(b, kSmallBatch);
-    } else {
-      NormBatch<kLargeBatch> b;
-      gather(b, kLargeBatch);
-    }
-  }
-  if (e == cudaSuccess) {
-    grad_norm_finish_kernel<<<1, kOptThreads, 0, st>>>(partial, parts, norm_out);
+  cudaError_t e = cudaSuccess;
+  if (!need) {
+    NormBatch<kSmallBatch> b;
+    gather(b, kSmallBatch, kNormClusterThreads * 8 * kNormUnits);
+    grad_norm_small_kernel<<<kNormCluster, kNormClusterThreads, 0, st>>>(b, norm_out);
     t_launches++;
     e = cudaGetLastError();
+  } else {
+    double* partial = reinterpret_cast<double*>(workspace);
+    int parts = 0;
+    const auto run = [&](auto& b, int most) {
+      gather(b, most, kOptThreads * 8 * kNormUnits);
+      if (!b.count) return;
+      const unsigned grid = std::min(b.chunks, (unsigned)kNormGrid);
+      b.partial = partial + parts;
+      e = launch_norm(b, grid, st);
+      parts += (int)grid;
+    };
+    while (i < n && e == cudaSuccess) {
+      if (n <= kSmallBatch) {
+        NormBatch<kSmallBatch> b;
+        run(b, kSmallBatch);
+      } else {
+        NormBatch<kLargeBatch> b;
+        run(b, kLargeBatch);
+      }
+    }
+    if (e == cudaSuccess) {
+      grad_norm_finish_kernel<<<1, kOptThreads, 0, st>>>(partial, parts, norm_out);
+      t_launches++;
+      e = cudaGetLastError();
+    }
   }
   if (e != cudaSuccess) return fail((int)e, "gradient norm launch failed: %s", cudaGetErrorString(e));
   return 0;

@@ -265,6 +265,7 @@ at::Tensor run_norm(PyObject* o, long* launches) {
     if (types[i] < 0) refuse(PyExc_TypeError, "gradients must be float32, bfloat16 or float16, got ", x.scalar_type());
     if (x.device() != dev) refuse(PyExc_RuntimeError, "gradients must be on one device, got ", x.device(), " beside ", dev);
   }
+  int64_t elements = 0;
   for (size_t i = 0; i < n; i++) {
     const at::Tensor* x = &grads[i];
     if (!dense(*x)) {
@@ -273,14 +274,18 @@ at::Tensor run_norm(PyObject* o, long* launches) {
     }
     at_[i] = x->const_data_ptr();
     numel[i] = x->numel();
+    elements += numel[i];
   }
   const at::TensorOptions options = at::TensorOptions().device(dev);
   at::Tensor norm = at::empty({}, options.dtype(at::kFloat));
-  const size_t need = g.grad_norm_workspace((int64_t)n);
-  const at::Tensor ws = at::empty({(int64_t)need}, options.dtype(at::kByte));
+  size_t need = 0;
+  if (const int rc = g.grad_norm_workspace((int64_t)n, elements, &need))
+    refuse(g.error, "flexsae_grad_norm failed (code ", rc, "): ", g.last_error());
+  at::Tensor ws;
+  if (need) ws = at::empty({(int64_t)need}, options.dtype(at::kByte));
   void* stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   float* out = norm.mutable_data_ptr<float>();
-  void* scratch = ws.mutable_data_ptr();
+  void* scratch = need ? ws.mutable_data_ptr() : nullptr;
   int rc = 0;
   Py_BEGIN_ALLOW_THREADS
   rc = g.grad_norm(at_.data(), numel.data(), types.data(), (int64_t)n, out, scratch, need, stream);

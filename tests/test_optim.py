@@ -163,16 +163,29 @@ def test_step_entries_refuse_before_any_launch(kw, text):
 
 def test_norm_entry_refuses_before_any_launch():
     lib = nv.load()
-    need = lib.flexsae_grad_norm_workspace_bytes(2)
-    assert need > 0 and lib.flexsae_grad_norm_workspace_bytes(-1) == 0 and lib.flexsae_grad_norm_workspace_bytes(1 << 17) == 0
+    size = ctypes.c_size_t()
 
-    def call(grads=(64, 128), numel=(4, 4), dtypes=(0, 1), n=2, out=512, ws=1024, ws_bytes=need):
+    def workspace(n, elements):
+        assert lib.flexsae_grad_norm_workspace_bytes(n, elements, ctypes.byref(size)) == 0
+        return size.value
+
+    assert lib.flexsae_grad_norm_workspace_bytes(-1, 8, ctypes.byref(size)) == -1
+    assert lib.flexsae_grad_norm_workspace_bytes(1 << 17, 8, ctypes.byref(size)) == -1
+    assert lib.flexsae_grad_norm_workspace_bytes(2, -1, ctypes.byref(size)) == -1
+    assert lib.flexsae_grad_norm_workspace_bytes(2, 8, None) == -1
+    assert workspace(16, 1 << 19) == 0                            # one cluster, no scratch memory
+    large = 1 << 20
+    need = workspace(2, large)
+    assert need > 0 and workspace(17, 8) > 0 and workspace(16, (1 << 19) + 1) > 0
+
+    def call(grads=(64, 1 << 30), numel=(large, 4), dtypes=(0, 1), n=2, out=512, ws=1024, ws_bytes=need):
         return lib.flexsae_grad_norm((ctypes.c_void_p * 2)(*grads), (ctypes.c_int64 * 2)(*numel), (ctypes.c_int32 * 2)(*dtypes), n, out, ws,
                                      ws_bytes, None), lib.flexsae_last_error().decode()
 
-    for kw, text in ((dict(n=-1), "tensors"), (dict(out=None), "null"), (dict(ws=None), "null"), (dict(ws=1028), "aligned"),
-                     (dict(ws_bytes=need - 1), "too small"), (dict(dtypes=(0, 5)), "dtype"), (dict(numel=(4, -4)), "numel"),
-                     (dict(grads=(64, 0)), "null"), (dict(grads=(66, 128)), "aligned"), (dict(grads=(64, 129)), "aligned")):
+    for kw, text in ((dict(n=-1), "tensors"), (dict(out=None), "null"), (dict(out=514), "norm_out"), (dict(ws=None), "workspace"),
+                     (dict(ws=1028), "aligned"), (dict(ws_bytes=need - 1), "too small"), (dict(dtypes=(0, 5)), "dtype"),
+                     (dict(numel=(large, -4)), "numel"), (dict(grads=(64, 0)), "null"), (dict(grads=(66, 128)), "aligned"),
+                     (dict(grads=(64, 129)), "aligned")):
         rc, err = call(**kw)
         assert rc < 0 and text in err, (kw, rc, err)
     assert lib.flexsae_grad_norm(None, None, None, 2, 512, 1024, need, None) == -1
@@ -268,7 +281,7 @@ NORM_TOL = 5 * U
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("n,offset", [(1, 0), (7, 0), (255, 1), (256, 0), (257, 3), (8191, 0), (8192, 0), (8193, 1), (100003, 0), (20_000_001, 0)])
+@pytest.mark.parametrize("n,offset", [(1, 0), (7, 0), (255, 1), (256, 0), (257, 3), (8191, 0), (8192, 0), (8193, 1), (100003, 0), (1 << 19, 0), ((1 << 19) + 1, 0), (20_000_001, 0)])
 def test_norm_of_one_tensor(dtype, n, offset):
     x = torch.randn(n + offset, generator=torch.Generator().manual_seed(n)).to(dtype).cuda()[offset:]
     want = float(x.double().square().sum().sqrt())
