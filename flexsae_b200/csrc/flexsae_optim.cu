@@ -22,7 +22,9 @@ constexpr int kNormUnits = 4;                               // units of 256 elem
 constexpr int kNormGrid = 148 * 8;
 constexpr int kNormCluster = 8, kNormClusterThreads = 512;
 constexpr int64_t kNormSmall = 1 << 19;                     // elements of a list for which one cluster is enough: four rounds
-constexpr int kSmallBatch = 16, kLargeBatch = 256;          // tensors of one launch
+// Tensors of one launch.  What a launch's arguments hold is paid for on the host: a step over 20 tensors takes the
+// caller 14 us with room for 32 of them and 23 us with room for 256; the GPU does not notice (3.2 us either way).
+constexpr int kSmallBatch = 32, kLargeBatch = 256;
 
 template <int N>
 struct NormBatch {

@@ -173,10 +173,10 @@ def test_norm_entry_refuses_before_any_launch():
     assert lib.flexsae_grad_norm_workspace_bytes(1 << 17, 8, ctypes.byref(size)) == -1
     assert lib.flexsae_grad_norm_workspace_bytes(2, -1, ctypes.byref(size)) == -1
     assert lib.flexsae_grad_norm_workspace_bytes(2, 8, None) == -1
-    assert workspace(16, 1 << 19) == 0                            # one cluster, no scratch memory
+    assert workspace(32, 1 << 19) == 0                            # one cluster, no scratch memory
     large = 1 << 20
     need = workspace(2, large)
-    assert need > 0 and workspace(17, 8) > 0 and workspace(16, (1 << 19) + 1) > 0
+    assert need > 0 and workspace(33, 8) > 0 and workspace(32, (1 << 19) + 1) > 0
 
     def call(grads=(64, 1 << 30), numel=(large, 4), dtypes=(0, 1), n=2, out=512, ws=1024, ws_bytes=need):
         return lib.flexsae_grad_norm((ctypes.c_void_p * 2)(*grads), (ctypes.c_int64 * 2)(*numel), (ctypes.c_int32 * 2)(*dtypes), n, out, ws,
@@ -291,7 +291,7 @@ def test_norm_of_one_tensor(dtype, n, offset):
 
 
 @gpu
-@pytest.mark.parametrize("count", [2, 16, 17, 256, 257, 600])
+@pytest.mark.parametrize("count", [2, 16, 17, 30, 31, 256, 257, 600])
 def test_norm_of_many_mixed_tensors(count):
     g = torch.Generator().manual_seed(count)
     dtypes = [torch.float32, torch.bfloat16, torch.float16]
