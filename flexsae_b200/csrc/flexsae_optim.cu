@@ -738,13 +738,17 @@ static int kind_of(const flexsae_optim_tensor& t) {
   return 1 + (t.param_dtype == FLEXSAE_F16 ? 4 : 0) + (t.grad_dtype == FLEXSAE_F32 ? 2 : 0) + (t.master ? 1 : 0);
 }
 
-// CTAs of `threads` that the GPU holds at the same time: the grid of a launch whose CTAs take every
-// gridDim-th unit, so that all of them run from the start and finish together.
+// CTAs of `threads` that the GPU holds at the same time, at most `most` per SM: the grid of a launch whose CTAs take
+// every gridDim-th chunk, so that all of them run from the start and finish together.  Asked for once (`known`).
 template <typename K>
-static unsigned resident_ctas(K kernel, int threads, int most = 32) {
+static cudaError_t resident_ctas(std::atomic<unsigned>& known, K kernel, int threads, int most, unsigned* ctas) {
+  *ctas = known.load(std::memory_order_relaxed);
+  if (*ctas) return cudaSuccess;
   int n = 0;
-  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0) != cudaSuccess || n < 1) n = 1;
-  return (unsigned)(std::min(n, most) * kOptSms);
+  if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0)) return e;
+  *ctas = (unsigned)(std::max(1, std::min(n, most)) * kOptSms);
+  known.store(*ctas, std::memory_order_relaxed);
+  return cudaSuccess;
 }
 
 // A launch that is set up while the kernel before it in the stream finishes; every kernel launched so waits for that
@@ -787,14 +791,20 @@ template <int N>
 static cudaError_t launch_adamw(const OptBatch<N>& b, int kind, int state_bits, cudaStream_t st) {
   const unsigned ctas = std::max(1u, b.chunks);
   cudaError_t e = cudaSuccess;
-#define CALL_ADAMW(P, G, M)                                                                             \
-  if (state_bits == 8) {                                                                                \
-    static const unsigned most = resident_ctas(adamw8_kernel<P, G, M, N>, kAdamw8Threads);              \
-    e = launch_early(adamw8_kernel<P, G, M, N>, std::min(ctas, most), kAdamw8Threads, b, st);           \
-  } else {                                                                                              \
-    constexpr int bytes = 8 * ((M ? 4 : sizeof(P)) + sizeof(G) + 8);                                    \
-    static const unsigned most = resident_ctas(adamw_kernel<P, G, M, N>, kAdamwThreads, kBytesInFlight / (kAdamwThreads * bytes)); \
-    e = launch_early(adamw_kernel<P, G, M, N>, std::min(ctas, most), kAdamwThreads, b, st);             \
+  unsigned most = 0;
+#define CALL_ADAMW(P, G, M)                                                                                  \
+  {                                                                                                          \
+    static std::atomic<unsigned> known[2];                                                                   \
+    if (state_bits == 8) {                                                                                   \
+      const auto kernel = adamw8_kernel<P, G, M, N>;                                                         \
+      e = resident_ctas(known[1], kernel, kAdamw8Threads, 32, &most);                                        \
+      if (e == cudaSuccess) e = launch_early(kernel, std::min(ctas, most), kAdamw8Threads, b, st);           \
+    } else {                                                                                                 \
+      constexpr int bytes = 8 * ((M ? 4 : sizeof(P)) + sizeof(G) + 8);                                       \
+      const auto kernel = adamw_kernel<P, G, M, N>;                                                          \
+      e = resident_ctas(known[0], kernel, kAdamwThreads, kBytesInFlight / (kAdamwThreads * bytes), &most);   \
+      if (e == cudaSuccess) e = launch_early(kernel, std::min(ctas, most), kAdamwThreads, b, st);            \
+    }                                                                                                        \
   }
   FLEXSAE_OPT_KINDS(kind, CALL_ADAMW)
 #undef CALL_ADAMW
@@ -863,13 +873,13 @@ static cudaError_t launch_rows(const RowArgs& a, int kind, cudaStream_t st) {
   const int teams = row_warps == 1 ? kRowTeams : 1, warps = row_warps * teams;
   const long long ctas = (a.rows + teams - 1) / teams;
   cudaError_t e = cudaSuccess;
-#define CALL_ROWS(P, G, M)                                                                                    \
-  {                                                                                                           \
+  unsigned most = 0;
+#define CALL_ROWS(P, G, M)                                                                                         \
+  {                                                                                                                \
     const auto kernel = warps <= 9 ? adamw_unit_rows_kernel<P, G, M, 288> : adamw_unit_rows_kernel<P, G, M, 1024>; \
-    static std::atomic<unsigned> most[33];                                                                    \
-    unsigned m = most[warps].load(std::memory_order_relaxed);                                                 \
-    if (!m) most[warps] = m = resident_ctas(kernel, warps * 32);                                              \
-    e = launch_early(kernel, (unsigned)std::min<long long>(ctas, m), warps * 32, a, st);                      \
+    static std::atomic<unsigned> known[33];                                                                        \
+    e = resident_ctas(known[warps], kernel, warps * 32, 32, &most);                                                \
+    if (e == cudaSuccess) e = launch_early(kernel, (unsigned)std::min<long long>(ctas, most), warps * 32, a, st);  \
   }
   FLEXSAE_OPT_KINDS(kind, CALL_ROWS)
 #undef CALL_ROWS

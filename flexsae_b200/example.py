@@ -11,6 +11,10 @@ HierarchicalTopK at K = 32, 64, 128 with F = 65536, D = 2304.
     python -m flexsae_b200.example --kind topk --dtype bf16 --B 4096 --K 128 --F 65536 --D 2304
     python -m flexsae_b200.example --table --B 4096
 
+``--optimizer adamw`` (or ``adamw8``, ``unit_rows``) adds a training step: the fused loss, its backward, the
+gradient norm and the optimizer step of ``flexsae_b200.optim`` on persistent parameters, beside the same
+step with ``torch.optim.AdamW(fused=True)`` and ``clip_grad_norm_``.
+
 ``--reference-path DIR`` also times the reference's own Triton kernels when a copy of its package
 directory (``torch-ext/flex_sae`` of corl-team/flexsae) is at hand; it is loaded from ``DIR`` under
 another module name and is not part of this library.
@@ -28,6 +32,7 @@ from typing import Callable, Dict, List, Optional
 import torch
 
 from . import hierarchical_sae_loss, topk_sae_loss, triton_hierarchical_sae_loss, triton_topk_sae_loss
+from .optim import AdamW
 
 DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 
@@ -88,6 +93,43 @@ def time_one(fn: Callable, B: int, K: int, F: int, D: int, dtype: torch.dtype, d
         del p
     return {"ms": statistics.fmean(times), "std": statistics.pstdev(times), "min": min(times),
             "gib": peak / 2 ** 30, "loss": float(loss)}
+
+
+OPTIMIZERS = {"adamw": {}, "adamw8": {"state_bits": 8}, "unit_rows": {"unit_rows": True}}
+
+
+def time_training(kind: str, B: int, K: int, F: int, D: int, dtype: torch.dtype, device: torch.device, warmup: int, iters: int,
+                  optimizer: str, max_norm: float = 1.0) -> Dict[str, float]:
+    """ms of one training step of the decoder (fused loss, backward, clipping, optimizer) with this library's
+    optimizer ("fused") and with torch's ("torch"), and of the optimizer's part alone."""
+    fn = triton_hierarchical_sae_loss if kind == "hier" else triton_topk_sae_loss
+    out: Dict[str, float] = {}
+    for name in ("fused", "torch"):
+        p = make_parameters(B, K, F, D, dtype, device)
+        trained = [p["weight"], p["bias"]]
+        if name == "fused":
+            groups = [{"params": [p["weight"]], **OPTIMIZERS[optimizer]}, {"params": [p["bias"]]}]
+            opt: torch.optim.Optimizer = AdamW(groups, lr=1e-4, max_norm=max_norm)
+        else:
+            opt = torch.optim.AdamW(trained, lr=1e-4, fused=True)
+        whole, part = [], []
+        for i in range(warmup + iters):
+            e = [torch.cuda.Event(enable_timing=True) for _ in range(3)]
+            e[0].record()
+            _step(fn, p)
+            e[1].record()
+            if name == "torch":
+                torch.nn.utils.clip_grad_norm_(trained, max_norm)
+            opt.step()
+            e[2].record()
+            _drop_grads(p)
+            torch.cuda.synchronize(device)
+            if i >= warmup:
+                whole.append(e[0].elapsed_time(e[2]))
+                part.append(e[1].elapsed_time(e[2]))
+        out[name], out[name + "_optimizer"] = statistics.fmean(whole), statistics.fmean(part)
+        del p, trained, opt
+    return out
 
 
 def load_reference_package(path: str):
@@ -156,6 +198,7 @@ def main(argv: Optional[List[str]] = None) -> Dict[str, object]:
     ap.add_argument("--compile", action="store_true", help="torch.compile(fullgraph=True) around the torch loss")
     ap.add_argument("--torch-chunk", type=int, default=0, help="rows per chunk of the torch loss (0 = whole batch)")
     ap.add_argument("--table", action="store_true", help="the README table: F=65536 D=2304 K in 32,64,128, bf16 unless --dtype")
+    ap.add_argument("--optimizer", default="none", choices=["none"] + sorted(OPTIMIZERS), help="also time a training step with this optimizer")
     ap.add_argument("--reference-path", default="", help="directory of the reference's flex_sae package: time its Triton kernels too")
     args = ap.parse_args(argv)
     reference = load_reference_package(args.reference_path) if args.reference_path else None
@@ -183,6 +226,11 @@ def main(argv: Optional[List[str]] = None) -> Dict[str, object]:
     print(f"fused kernels (ours): {f['ms']:.4f} ± {f['std']:.4f} ms   peak {f['gib']:.2f} GiB")
     print(f"torch loss:           {t['ms']:.4f} ± {t['std']:.4f} ms   peak {t['gib']:.2f} GiB")
     print(f"speed-up: {t['ms'] / f['ms']:.2f}x")
+    if args.optimizer != "none":
+        s = time_training(args.kind, args.B, args.K, args.F, args.D, DTYPES[args.dtype], device, args.warmup, args.iters, args.optimizer)
+        r["training"] = s
+        print(f"training step ({args.optimizer}, clipped): {s['fused']:.4f} ms, of it optimizer {s['fused_optimizer']:.4f} ms;   "
+              f"with torch's fused AdamW {s['torch']:.4f} ms, of it optimizer {s['torch_optimizer']:.4f} ms")
     if "reference_triton" in r:
         q = r["reference_triton"]
         print(f"reference Triton:     {q['ms']:.4f} ± {q['std']:.4f} ms   peak {q['gib']:.2f} GiB   ({q['ms'] / f['ms']:.2f}x ours)")

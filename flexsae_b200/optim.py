@@ -4,8 +4,9 @@ AdamW on a decoder whose rows are kept at unit length.
 The reference ends at the gradients (torch-ext/flex_sae/hierarchical_kernels.py:288-299); its callers
 take the step with the optimizer of their choice.  Here one launch updates all tensors of a model:
 
-    opt = flexsae_b200.optim.AdamW([{"params": [w_enc, b_enc, b_dec]},
-                                    {"params": [w_dec], "unit_rows": True}], lr=1e-4, max_norm=1.0)
+    from flexsae_b200 import optim
+    opt = optim.AdamW([{"params": [w_enc, b_enc, b_dec]},
+                       {"params": [w_dec], "unit_rows": True}], lr=1e-4, max_norm=1.0)
     loss.backward()
     opt.step()
     opt.zero_grad()

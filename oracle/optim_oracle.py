@@ -62,10 +62,10 @@ def mix(x):
     return x ^ (x >> np.uint64(16))
 
 
-def random_bits(seed: int, t: int, index: int, n: int):
-    """(20 bits for m, 21 bits for v) of the n elements of tensor ``index``."""
+def random_bits(seed: int, t: int, index: int, n: int, first: int = 0):
+    """(20 bits for m, 21 bits for v) of the n elements from ``first`` on of tensor ``index``."""
     key = int(mix(int(mix(int(mix(t & 0xFFFFFFFF)) + index)) + seed))
-    e = np.arange(n, dtype=np.uint64)
+    e = np.arange(first, first + n, dtype=np.uint64)
     pair = e >> np.uint64(1)
     h = mix((pair & np.uint64(0xFFFFFFFF)) ^ ((np.uint64(key) + (pair >> np.uint64(32))) & np.uint64(0xFFFFFFFF)))
     odd = (e & np.uint64(1)).astype(bool)
@@ -111,9 +111,10 @@ def moments32(g: np.ndarray, m8, m_scale, v8, v_scale, betas=(0.9, 0.999), clip:
         return f(betas[0]) * m + f(1 - betas[0]) * g, f(betas[1]) * v + f(1 - betas[1]) * (g * g)
 
 
-def adamw8_states(g, m8, m_scale, v8, v_scale, t: int, seed: int, index: int, betas=(0.9, 0.999), clip: float = 1.0):
-    """(m, v, m8, m_scale, v8, v_scale) after the step: the 32-bit moments and what is stored of them."""
+def adamw8_states(g, m8, m_scale, v8, v_scale, t: int, seed: int, index: int, betas=(0.9, 0.999), clip: float = 1.0, first: int = 0):
+    """(m, v, m8, m_scale, v8, v_scale) after the step: the 32-bit moments and what is stored of them.  The arrays are
+    the tensor's elements from ``first`` (a multiple of the block) on."""
     m, v = moments32(g, m8, m_scale, v8, v_scale, betas, np.float32(clip))
-    rm, rv = random_bits(seed, t, index, len(g))
+    rm, rv = random_bits(seed, t, index, len(g), first)
     sm, sv = scales(m, 448.0), scales(v, 57344.0)
     return m, v, codes(m, sm, rm, "m"), sm, codes(v, sv, rv, "v"), sv

@@ -575,8 +575,110 @@ def test_adamw8_extreme_gradients(scale):
     assert torch.isfinite(x[0]).all()
 
 
+@gpu
+@pytest.mark.parametrize("eps", [1e-15, 1e-30])
+@pytest.mark.parametrize("entry", ["adamw", "adamw8", "rows"])
+def test_an_eps_beside_which_tiny_roots_count(eps, entry):
+    """Gradients of 1e-17 and below, whose squares are subnormal or zero in 32 bits, with an eps of their size or less.
+    A square rounded to a multiple of 2^-149 is off by 2^-150, the rounded product (1 - b2) g^2 by as much again; the root of
+    v is then off by at most sqrt(2^-148), which the bound takes beside the usual ones."""
+    x = make8((3, 256), torch.float32, 31) if entry == "adamw8" else make((3, 256), torch.float32, 31)
+    w = x[0]
+    w.copy_(torch.nn.functional.normalize(w, dim=1))
+    g = torch.Generator().manual_seed(2)
+    x[1].copy_(torch.randn(3, 256, generator=g) * torch.tensor([1e-14, 1e-17, 1e-19])[:, None])
+    states = (x[2], x[4]) if entry == "adamw8" else (x[2], x[3])
+    for t in states:
+        t.view(torch.uint8).zero_()
+    if entry == "adamw8":
+        x[3].zero_(), x[5].zero_()
+    b, grad = f64(w), f64(x[1])
+    kw = dict(lr=1e-3, betas=(0.9, 0.99), eps=eps, weight_decay=0.0)
+    if entry == "adamw8":
+        optim.adamw8_step(*[[t] for t in x[:6]], steps_in(0), **kw)
+    else:
+        (optim.adamw_step if entry == "adamw" else optim.adamw_unit_rows_step)(*[[t] for t in x[:4]], steps_in(0), **kw)
+    if entry == "rows":                                  # the first row's squares are ordinary numbers: the usual bounds
+        want = orc.adamw(b, grad, 0 * b, 0 * b, 1, 1e-3, (0.9, 0.99), eps, 0.0, unit_rows=True)
+        ep, em, ev = rows_bounds((b, grad, 0 * b, 0 * b), want, 1, 1e-3, 1.0, (0.9, 0.99), eps, 0.0)
+        close(w[0], want[0][0], ep[0], "param"), close(x[2][0], want[1][0], em[0], "m"), close(x[3][0], want[2][0], ev[0], "v")
+        assert torch.isfinite(w).all() and np.abs(np.linalg.norm(f64(w), axis=1) - 1).max() <= 16 * U
+        return
+    v = 0.01 * grad * grad
+    tiny = 2.0 ** -148
+    step = lambda v: 1e-3 * np.abs(grad) / (np.sqrt(np.maximum(v, 0)) / np.sqrt(0.01) + eps)  # noqa: E731
+    low, high = step(v * (1 + 64 * U) + tiny) * (1 - 128 * U), step(v * (1 - 64 * U) - tiny) * (1 + 128 * U)
+    moved = np.abs(b - f64(w))
+    slack = 2 * U * np.abs(b)
+    assert np.all(moved >= low - slack) and np.all(moved <= high + slack)
+
+
+@gpu
+def test_results_do_not_depend_on_alignment():
+    """The fast path for aligned tensors and the general one give the same bits, also next to a NaN."""
+    for dtype, grad_dtype, master in KINDS:
+        a, b = (make((5000,), dtype, 3, master, grad_dtype, off) for off in (0, 1))
+        for x in (a, b):
+            optim.adamw_step(*[[t] for t in x[:4]], steps_in(5), lr=1e-3, masters=[x[4]])
+        assert all(torch.equal(s, t) for s, t in zip(a[:4], b[:4]))
+        a, b = (make8((5000,), dtype, 3, master, off) for off in (0, 1))
+        for x in (a, b):
+            x[1][[700, 701, 4000]] = math.nan
+            for _ in range(2):
+                optim.adamw8_step(*[[t] for t in x[:6]], steps_in(5), lr=1e-3, masters=[x[6]])
+        assert all(torch.equal(s.view(torch.uint8) if s.dtype in optim.STATE8_DTYPES else s.nan_to_num(7.0),
+                               t.view(torch.uint8) if t.dtype in optim.STATE8_DTYPES else t.nan_to_num(7.0)) for s, t in zip(a[:6], b[:6]))
+        a, b = (make((40, 128), dtype, 3, master, grad_dtype, off) for off in (0, 1))
+        for x in (a, b):
+            optim.adamw_unit_rows_step(*[[t] for t in x[:4]], steps_in(5), lr=1e-3, masters=[x[4]])
+        for s, t in zip(a[:4], b[:4]):                      # the sums over a row are taken in another order
+            assert torch.allclose(s.float(), t.float(), rtol=1e-2 if s.dtype != torch.float32 else 1e-4, atol=1e-6)
+
+
+@gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_tensors_of_more_than_two_to_the_31_elements(bits):
+    """Every kind of offset passes 32 bits; the first, the middle and the last elements are the oracle's."""
+    n = 2 ** 31 + 256 * 9 + 77
+    g = torch.Generator(device="cuda").manual_seed(1)
+    spots = [0, 2 ** 30 - 512, 2 ** 31 - 512, n - 77 - 1024]          # multiples of 256
+    p, grad = (torch.zeros(n, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+    if bits == 32:
+        state = [torch.zeros(n, device="cuda") for _ in range(2)]
+    else:
+        state = [torch.zeros(n, dtype=d, device="cuda") for d in optim.STATE8_DTYPES]
+        scale = [torch.zeros(optim.state8_blocks(n), device="cuda") for _ in range(2)]
+    for s in spots:
+        p[s:s + 1024] = torch.randn(min(1024, n - s), generator=g, device="cuda").bfloat16()
+        grad[s:s + 1024] = torch.randn(min(1024, n - s), generator=g, device="cuda").bfloat16()
+    grad[-77:] = torch.randn(77, generator=g, device="cuda").bfloat16()
+    parts = [(s, min(s + 1024, n)) for s in spots] + [(n - 77, n)]
+    before = [(f64(p[a:b]), grad[a:b].float().cpu().numpy()) for a, b in parts]
+    norm = optim.grad_norm([grad])
+    want = math.sqrt(sum(float((x[1].astype(np.float64) ** 2).sum()) for x in before))
+    assert abs(float(norm) - want) <= NORM_TOL * want
+    step = steps_in(0)
+    if bits == 32:
+        optim.adamw_step([p], [grad], [state[0]], [state[1]], step, lr=1e-2)
+    else:
+        optim.adamw8_step([p], [grad], [state[0]], [scale[0]], [state[1]], [scale[1]], step, lr=1e-2, seed=11)
+    for (a, b), (q, x) in zip(parts, before):
+        zero = np.zeros(b - a)
+        exact = orc.adamw(q, x, zero, zero, 1, 1e-2)
+        bound = bounds((q, x, zero, zero), exact, 1, 1e-2, (0.9, 0.999), 1e-8, 1.0)
+        check_params(p[a:b], None, exact[0], bound[0], torch.bfloat16)
+        if bits == 32:
+            close(state[0][a:b], exact[1], bound[1], "m"), close(state[1][a:b], exact[2], bound[2], "v")
+        else:
+            blocks = slice(a // 256, -(-b // 256))
+            none, nothing = np.zeros(b - a, dtype=np.uint8), np.zeros(-(-(b - a) // 256), dtype=np.float32)
+            _, _, m8, ms, v8, vs = orc.adamw8_states(x, none, nothing, none, nothing, 1, 11, 0, first=a)
+            assert np.array_equal(bytes_of(state[0][a:b]), m8) and np.array_equal(bytes_of(state[1][a:b]), v8)
+            assert np.array_equal(scale[0][blocks].cpu().numpy(), ms) and np.array_equal(scale[1][blocks].cpu().numpy(), vs)
+
+
 # ---- GPU: unit rows -------------------------------------------------------------------------------------
-def rows_bounds(b, want, t, lr, clip):
+def rows_bounds(b, want, t, lr, clip, betas=(0.9, 0.999), eps=1e-8, decay=0.01):
     """As ``bounds``, for the row form.  A sum over a row is off by at most (8 + 10 + 1) u of the sum of its absolute terms
     (eight in a row, five and five levels of a tree), so the projection moves g by (40 u) |along|abs |p| + 3 u of its own terms;
     a new row is divided by its length (12 u of the row, and the errors of its elements once more through the length)."""
@@ -586,14 +688,14 @@ def rows_bounds(b, want, t, lr, clip):
     along = np.divide(np.sum(np.abs(g * p), axis=1, keepdims=True), square, out=np.zeros_like(square), where=square > 0)
     eg = U * (48 * along * np.abs(p) + 8 * np.abs(g))
     projected = np.abs(g) + along * np.abs(p)
-    em = U * (3 * 0.9 * np.abs(m) + 4 * 0.1 * projected) + 0.1 * eg
-    ev = U * (3 * 0.999 * np.abs(v) + 5 * 0.001 * projected ** 2) + 0.001 * (2 * projected * eg + eg * eg)
+    em = U * (3 * betas[0] * np.abs(m) + 4 * (1 - betas[0]) * projected) + (1 - betas[0]) * eg
+    ev = U * (3 * betas[1] * np.abs(v) + 5 * (1 - betas[1]) * projected ** 2) + (1 - betas[1]) * (2 * projected * eg + eg * eg)
     # errors of the step, to first order around the exact moments, the denominator at its smallest
-    denom = np.sqrt(np.maximum(want[2] - ev, 0)) / math.sqrt(1 - 0.999 ** t) + 1e-8
-    rate = lr / (1 - 0.9 ** t)
-    upper = np.sqrt(want[2] + ev) / math.sqrt(1 - 0.999 ** t) + 1e-8
+    denom = np.sqrt(np.maximum(want[2] - ev, 0)) / math.sqrt(1 - betas[1] ** t) + eps
+    rate = lr / (1 - betas[0] ** t)
+    upper = np.sqrt(want[2] + ev) / math.sqrt(1 - betas[1] ** t) + eps
     ep = 4 * U * np.abs(p) + rate * (np.abs(want[1]) * (1 / denom - 1 / upper) + em / denom) + 24 * U * rate * np.abs(want[1]) / denom
-    new = p * (1 - lr * 0.01) - rate * want[1] / (np.sqrt(want[2]) / math.sqrt(1 - 0.999 ** t) + 1e-8)
+    new = p * (1 - lr * decay) - rate * want[1] / (np.sqrt(want[2]) / math.sqrt(1 - betas[1] ** t) + eps)
     length = np.sqrt(np.sum(new * new, axis=1, keepdims=True))
     length = np.where(length > 0, length, 1)
     through = np.sum(np.abs(want[0]) * ep, axis=1, keepdims=True) / length
@@ -676,6 +778,71 @@ def test_captured_steps_replay_like_eager_ones(bits):
 
 
 @gpu
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing has to be warmed up: every kernel is first launched inside the capture."""
+    import subprocess
+    import sys
+
+    code = """
+import torch
+from flexsae_b200 import optim
+ts = [[torch.ones(40, 64, device='cuda') for _ in range(2)] for _ in range(4)]
+big = torch.ones(1 << 20, device='cuda')
+m8 = [torch.zeros(40, 64, dtype=d, device='cuda') for d in optim.STATE8_DTYPES]
+s8 = [torch.zeros(10, device='cuda') for _ in range(2)]
+step = torch.zeros((), dtype=torch.int64, device='cuda')
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    norm = optim.grad_norm(ts[1] + [big])
+    small = optim.grad_norm(ts[1])
+    optim.adamw_step(*ts, step, lr=1e-3, norm=norm, max_norm=1.0)
+    optim.adamw_unit_rows_step(*ts, step, lr=1e-3, norm=small, max_norm=1.0)
+    optim.adamw8_step(ts[0], ts[1], [m8[0], m8[0].clone()], [s8[0], s8[0].clone()], [m8[1], m8[1].clone()], [s8[1], s8[1].clone()], step, lr=1e-3)
+for _ in range(3):
+    graph.replay()
+torch.cuda.synchronize()
+assert int(step) == 9 and abs(float(norm) - (2 * 2560 + (1 << 20)) ** 0.5) < 1e-3 and abs(float(small) - 5120 ** 0.5) < 1e-4
+print('captured')
+"""
+    import os
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stdout + r.stderr
+
+
+@gpu
+def test_two_captured_graphs_replay_side_by_side():
+    """Two graphs captured one after the other from the same stream hold their own scratch memory."""
+    sets = [make((3000, 333), torch.bfloat16, 70 + k) for k in range(2)]
+    grads = [[x[1], torch.randn(1 << 20, generator=torch.Generator().manual_seed(k)).cuda()] for k, x in enumerate(sets)]
+    steps, want = [steps_in(0), steps_in(0)], []
+    for k, x in enumerate(sets):
+        y = [t.clone() for t in x[:4]]
+        count = steps_in(0)
+        for _ in range(8):
+            norm = optim.grad_norm(grads[k])
+            optim.adamw_step(*[[t] for t in y], count, lr=1e-3, norm=norm, max_norm=1.0)
+        want.append(y)
+    graphs = []
+    for k, x in enumerate(sets):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            norm = optim.grad_norm(grads[k])
+            optim.adamw_step(*[[t] for t in x[:4]], steps[k], lr=1e-3, norm=norm, max_norm=1.0)
+        graphs.append(graph)
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for x, y, count in zip(sets, want, steps):
+        assert int(count) == 8 and all(torch.equal(a, b) for a, b in zip(x[:4], y))
+
+
+@gpu
 def test_steps_on_two_streams_do_not_disturb_each_other():
     def run(streams):
         sets = [make((4000, 257), torch.float32, 20 + k) for k in range(2)]
@@ -745,7 +912,7 @@ def test_training_run_encoder_selection_loss_and_step(dtype, bits, master):
             assert int(state["step"]) == t
             if rows or bits == 32:
                 b = (before[k], grads[k], m[k], v[k])
-                ep, em, ev = rows_bounds(b, want, t, lr, clip) if rows else bounds(b, want, t, lr, (0.9, 0.999), 1e-6, clip)
+                ep, em, ev = rows_bounds(b, want, t, lr, clip, eps=1e-6) if rows else bounds(b, want, t, lr, (0.9, 0.999), 1e-6, clip)
                 close(state["exp_avg"], want[1], em, k)
                 close(state["exp_avg_sq"], want[2], ev, k)
                 m[k], v[k] = f64(state["exp_avg"]), f64(state["exp_avg_sq"])
@@ -828,3 +995,13 @@ def test_skip_nonfinite_and_copies_of_the_optimizer():
         q.grad = torch.ones_like(q)
         other.step()
         assert other.skip_nonfinite and int(other.state[q]["step"]) == 2 and not torch.equal(q, kept)
+
+
+@gpu
+@pytest.mark.parametrize("optimizer", ["adamw", "adamw8", "unit_rows"])
+def test_example_times_a_training_step(optimizer, capsys):
+    from flexsae_b200 import example
+
+    r = example.main(["--B", "64", "--K", "32", "--F", "1024", "--D", "256", "--iters", "2", "--warmup", "1", "--optimizer", optimizer])
+    assert 0 < r["training"]["fused_optimizer"] < r["training"]["fused"] and r["training"]["torch"] > 0
+    assert "training step" in capsys.readouterr().out
