@@ -65,6 +65,7 @@ constexpr unsigned long long kStepMask = (1ull << 40) - 1;
 
 // Waits until the kernels before this one in the stream have finished and their results can be seen.
 __device__ __forceinline__ void opt_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // The numbers that are the same for every element of a step.  False: the gradient norm is not finite
 // and the step does not take place.
 __device__ __forceinline__ bool opt_coefs(const OptScalars& s, OptCoefs& c) {

@@ -88,7 +88,7 @@ def adamw8_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_s
     the rounding is right on average (rounding to nearest would never move a second moment, which a
     step changes by a thousandth).  The random bits are a function of (seed, t, position in the list,
     element).  A second moment is stored as at least 2^-16 of its scale.  An infinity or a NaN
-    stays with its own element."""
+    stays with its own element (a first moment's infinity as a NaN, which e4m3 has in its place)."""
     _step(_ADAMW8, params, grads, exp_avgs, exp_avg_scales, exp_avg_sqs, exp_avg_sq_scales, masters, step, lr, betas, eps,
           weight_decay, norm, max_norm, seed)
 
@@ -99,7 +99,7 @@ def adamw_unit_rows_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, 
                          max_norm: Optional[float] = None) -> None:
     """``adamw_step`` for decoders [F, D] (contiguous, D up to 8192) whose rows are kept at unit length: the
     gradient's component along its row is taken out first (g -= (g.w / w.w) w), and after the step
-    the row is divided by its length.  A row of zeros stays one."""
+    the row is divided by its length.  A row of zeros stays one; an infinity or NaN in a gradient reaches its row."""
     _step(_UNIT_ROWS, params, grads, exp_avgs, None, exp_avg_sqs, None, masters, step, lr, betas, eps, weight_decay, norm, max_norm)
 
 
@@ -207,20 +207,28 @@ class AdamW(torch.optim.Optimizer):
     def __getstate__(self) -> dict:
         return {**super().__getstate__(), "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite, "norm": None}
 
+    def __setstate__(self, state: dict) -> None:
+        super().__setstate__(state)
+        for group in self.param_groups:                 # a state of torch.optim.AdamW knows fewer options
+            for name, value in self.defaults.items():
+                group.setdefault(name, value)
+
     def load_state_dict(self, state_dict: dict) -> None:
-        """Restores a ``state_dict``: the states keep their own types (the base class would turn them into the
-        parameters'), and parameters of a group that stand at the same step share their count again."""
+        """Restores a ``state_dict``, also one of ``torch.optim.AdamW`` for 32-bit states: the states keep their own types
+        (the base class would turn them into the parameters'), and parameters of a group that stand at the same step
+        share their count again."""
         super().load_state_dict(state_dict)
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
-        params = [p for group in self.param_groups for p in group["params"]]
-        for i, p in zip(saved_ids, params):
+        params = [(p, group) for group in self.param_groups for p in group["params"]]
+        for i, (p, group) in zip(saved_ids, params):
             for name, value in state_dict["state"].get(i, {}).items():
                 if name == "step":
                     self.state[p][name] = torch.as_tensor(value).to(device=p.device, dtype=torch.int64).clone()
                 elif name.endswith("_scale"):
                     self.state[p][name] = value.to(p.device).clone()
                 else:
-                    kept = torch.empty_like(p, dtype=value.dtype, memory_format=torch.preserve_format)
+                    dtype = torch.float32 if group["state_bits"] == 32 else value.dtype
+                    kept = torch.empty_like(p, dtype=dtype, memory_format=torch.preserve_format)
                     self.state[p][name] = kept.copy_(value)
         for group in self.param_groups:
             counts: Dict[int, torch.Tensor] = {}

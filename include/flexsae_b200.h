@@ -306,7 +306,7 @@ int flexsae_loss_fwd_static_scratch(int kind, const int64_t* indices, const void
  * (torch-ext/flex_sae/hierarchical_kernels.py:288-299) and leaves the step to its caller.
  *
  * A step takes a host array of tensors.  All pointers in it are device pointers, aligned to their
- * elements; 16-byte alignment (8 for 8-bit states) is faster.  Elements are taken in memory order, so
+ * elements; aligned to eight elements (32, 16 or 8 bytes) they are faster.  Elements are taken in memory order, so
  * the tensors of one entry have the same layout.  An entry with numel 0 is passed over.  Memory that
  * a step writes must not overlap anything else in its list: this is checked, and refused.
  */

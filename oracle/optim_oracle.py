@@ -47,10 +47,10 @@ E4M3, E5M2 = grid(3, 7, 127), grid(2, 15, 124)
 
 
 def widen(codes: np.ndarray, kind: str) -> np.ndarray:
-    """float32 values of uint8 codes ("m": e4m3, "v": e5m2), NaN for 0x7f."""
+    """float32 values of uint8 codes ("m": e4m3, "v": e5m2), NaN for 0x7f and infinity for an e5m2 0x7c."""
     table = E4M3 if kind == "m" else E5M2
     low = codes & 0x7F
-    x = np.where(low < len(table), table[np.minimum(low, len(table) - 1)], np.nan).astype(np.float32)
+    x = np.where(low < len(table), table[np.minimum(low, len(table) - 1)], np.where((low == 0x7C) & (kind == "v"), np.inf, np.nan)).astype(np.float32)
     return np.where(codes & 0x80, -x, x)
 
 
@@ -77,11 +77,15 @@ def _by_block(x: np.ndarray) -> np.ndarray:
 
 
 def scales(x: np.ndarray, largest_code: float) -> np.ndarray:
-    """float32 scale of every block: its largest finite absolute value / the format's largest number, 2^-20 larger."""
+    """float32 scale of every block: its largest finite absolute value / the format's largest number, 2^-20 larger.  A
+    block of second moments whose finite values give none but that holds an infinity has the least one."""
     factor = np.float32((1.0 / largest_code) * (1.0 + 2.0 ** -20))
     a = np.abs(_by_block(x))
     s = np.max(np.where(np.isfinite(a), a, np.float32(0)), axis=1).astype(np.float32) * factor
-    return np.where(s >= np.float32(2.0 ** -126), s, np.float32(0))
+    s = np.where(s >= np.float32(2.0 ** -126), s, np.float32(0))
+    if largest_code == 57344.0:
+        s = np.where((s == 0) & np.any(a == np.inf, axis=1), np.float32(2.0 ** -126), s)
+    return s.astype(np.float32)
 
 
 def codes(x: np.ndarray, scale: np.ndarray, random: np.ndarray, kind: str) -> np.ndarray:
@@ -95,7 +99,7 @@ def codes(x: np.ndarray, scale: np.ndarray, random: np.ndarray, kind: str) -> np
     if kind == "v":
         size = np.fmax(size, np.float32(2.0 ** -128))
     c = (size.view(np.uint32).astype(np.uint64) + random.astype(np.uint64)) >> np.uint64(drop)
-    c = np.where(np.isfinite(x), c, 0x7F).astype(np.uint8)
+    c = np.where(np.isfinite(x), c, np.where((x == np.inf) & (kind == "v"), 0x7C, 0x7F)).astype(np.uint8)
     if kind == "m":
         c = np.where(np.isfinite(x) & np.signbit(y), c | 0x80, c)
     return c.astype(np.uint8)

@@ -555,7 +555,28 @@ def test_adamw8_nonfinite_values_stay_with_their_elements():
     keep = torch.ones(768, dtype=torch.bool, device="cuda")
     keep[[300, 301]] = False
     assert torch.equal(x[0][keep], sets[1][0][keep]) and not torch.isfinite(x[0][~keep]).any()
-    assert torch.isnan(x[2].float()[[300, 301]]).all() and torch.isnan(x[4].float()[[300, 301]]).all()
+    assert torch.isnan(x[2].float()[[300, 301]]).all() and torch.isnan(x[4].float()[300]) and float(x[4].float()[301]) == math.inf
+
+
+@gpu
+@pytest.mark.parametrize("alone", [False, True])
+def test_adamw8_second_moment_that_overflows_stays_infinite(alone):
+    """As with 32-bit states: the element's parameter stands still from then on and nothing becomes a NaN."""
+    x = make8((512,), torch.float32, 13)
+    for k in (2, 4):
+        x[k].view(torch.uint8).zero_()
+        x[k + 1].zero_()
+    x[1].copy_(torch.randn(512, generator=torch.Generator().manual_seed(1)) * (0 if alone else 1e-3))
+    x[1][300] = 1e30
+    kept, step = x[0].clone(), steps_in(0)
+    for t in range(3):
+        before = [x[1].cpu().numpy(), bytes_of(x[2]), x[3].cpu().numpy(), bytes_of(x[4]), x[5].cpu().numpy()]
+        optim.adamw8_step(*[[x[j]] for j in range(6)], step, lr=1e-3, weight_decay=0.0, seed=3)
+        _, _, m8, ms, v8, vs = orc.adamw8_states(*before, t + 1, 3, 0)
+        assert np.array_equal(bytes_of(x[2]), m8) and np.array_equal(bytes_of(x[4]), v8)
+        assert np.array_equal(x[3].cpu().numpy(), ms) and np.array_equal(x[5].cpu().numpy(), vs)
+        assert bytes_of(x[4])[300] == 0x7C and torch.isfinite(x[0]).all() and float(x[0][300]) == float(kept[300])
+        x[1][300] = 0
 
 
 @gpu
@@ -959,6 +980,31 @@ def test_state_dict_continues_the_run(bits):
         assert torch.equal(p, q)
         for name, value in first.state[p].items():
             assert torch.equal(value.view(torch.uint8) if value.dim() else value, second.state[q][name].view(torch.uint8) if value.dim() else second.state[q][name])
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_state_of_torchs_adamw_is_taken_over(dtype):
+    ps, qs = ([torch.nn.Parameter(p.detach().clone()) for p in make_sae(64, 40, dtype).values()] for _ in range(2))
+    theirs, ours = torch.optim.AdamW(ps, lr=1e-2), optim.AdamW(qs, lr=5e-3, max_norm=1e9)
+    for t in range(3):
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(t)).to(dtype).cuda()
+        theirs.step()
+    with torch.no_grad():
+        for p, q in zip(ps, qs):
+            q.copy_(p)
+            q.grad = p.grad.clone()
+    ours.load_state_dict(theirs.state_dict())
+    assert ours.param_groups[0]["lr"] == 1e-2 and ours.param_groups[0]["state_bits"] == 32
+    before = [[f64(t) for t in (q, q.grad, ours.state[q]["exp_avg"], ours.state[q]["exp_avg_sq"])] for q in qs]
+    ours.step()
+    for q, b in zip(qs, before):
+        want = orc.adamw(*b, 4, 1e-2)
+        ep, em, ev = bounds(b, want, 4, 1e-2, (0.9, 0.999), 1e-8, 1.0)
+        assert int(ours.state[q]["step"]) == 4 and ours.state[q]["exp_avg"].dtype == torch.float32
+        check_params(q, None, want[0], ep, dtype)
+        close(ours.state[q]["exp_avg"], want[1], em, "m"), close(ours.state[q]["exp_avg_sq"], want[2], ev, "v")
 
 
 @gpu
