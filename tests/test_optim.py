@@ -883,6 +883,52 @@ def test_steps_on_two_streams_do_not_disturb_each_other():
 
 
 @gpu
+@pytest.mark.parametrize("entry", ["norm", "adamw", "adamw8", "rows"])
+def test_calls_wait_for_the_copies_and_fills_before_them(entry):
+    """Launches are set up early; what they read may still be on its way, from the host, on the device or from another stream."""
+    F, D = 6000, 4096
+    host = torch.randn(F, D, generator=torch.Generator().manual_seed(3)).pin_memory()
+    source = host.cuda()
+    side = torch.cuda.Stream()
+
+    def run(bring):
+        p, grad = torch.ones(F, D, device="cuda"), torch.full((F, D), 7.0, device="cuda")
+        m, v = (torch.zeros(F, D, device="cuda") for _ in range(2))
+        m8, v8 = (torch.zeros(F, D, dtype=d, device="cuda") for d in optim.STATE8_DTYPES)
+        scales = [torch.zeros(F * D // 256, device="cuda") for _ in range(2)]
+        step = steps_in(0)
+        torch.cuda.synchronize()
+        bring(grad)
+        if entry == "norm":
+            out = [optim.grad_norm([grad])]
+        elif entry == "adamw8":
+            optim.adamw8_step([p], [grad], [m8], [scales[0]], [v8], [scales[1]], step, lr=1e-2)
+            out = [p, m8.view(torch.uint8), scales[1]]
+        else:
+            (optim.adamw_step if entry == "adamw" else optim.adamw_unit_rows_step)([p], [grad], [m], [v], step, lr=1e-2)
+            out = [p, m, v]
+        grad.fill_(math.nan)                     # and what follows waits for them
+        torch.cuda.synchronize()
+        return out
+
+    def from_side(grad):
+        with torch.cuda.stream(side):
+            grad.copy_(source)
+        torch.cuda.current_stream().wait_stream(side)
+
+    def zeroed(grad):
+        grad.zero_()
+        grad.add_(source)
+
+    want = run(lambda grad: (grad.copy_(source), torch.cuda.synchronize()))
+    for bring in (lambda grad: grad.copy_(host, non_blocking=True), lambda grad: grad.copy_(source), from_side, zeroed):
+        assert all(torch.equal(a, b) for a, b in zip(run(bring), want))
+    cleared = run(lambda grad: grad.zero_())
+    if entry == "norm":
+        assert float(cleared[0]) == 0
+
+
+@gpu
 def test_autograd_sees_that_a_parameter_changed():
     p = torch.randn(8, device="cuda", requires_grad=True)
     loss = (p * p).sum()
