@@ -29,7 +29,7 @@ NVCC_FLAGS = [
 ]
 #: sources compiled without ``--use_fast_math``: the optimizer's 8-bit states are rounded on bit patterns
 #: that flush-to-zero would destroy, and its 32-bit update uses IEEE division and square root
-IEEE_SOURCES = ("flexsae_optim.cu",)
+IEEE_SOURCES = ("flexsae_optim.cu", "flexsae_optim_rows.cu")
 
 
 def _sources():

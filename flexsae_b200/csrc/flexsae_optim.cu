@@ -153,17 +153,6 @@ __global__ void __cluster_dims__(kNormCluster, 1, 1) __launch_bounds__(kNormClus
 // Bound by HBM: 302 M bf16 parameters in 1.03 ms (99 % of the measured copy rate), 268 M fp32 in 1.13 ms (102 %).
 constexpr int kAdamwThreads = 128, kAdamw8Threads = 256;
 
-__device__ __forceinline__ float sqrt_approx(float x) {
-  float y;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float rcp_approx(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // The chunks of all tensors (a unit for every one of a CTA's warps) are dealt out to the CTAs in turn.  Step is told about
 //   full(first, end, stride)  its complete, aligned chunks of a tensor, which lie in one span of 2^31 elements;
 //                             answers the first one that it has not done (for this warp), from which on units go to
@@ -190,47 +179,6 @@ __device__ __forceinline__ void opt_walk(const OptBatch<N>& b, Step& step) {
       if ((long long)u * kOptBlock < t.numel) step.part(u);
     }
     c += ((last - 1 - c) / gridDim.x + 1) * gridDim.x;
-  }
-}
-
-// One step of two elements, the same bits wherever it is taken: the moments, then the parameter.  Products that
-// are added to something are multiply-adds with a -0 that the compiler cannot see: it would contract a packed
-// product and a packed sum, which are to be rounded one by one (see opt_moments).  Root and reciprocal are
-// approximate, 2 u each: they only reach the parameter.
-__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
-
-__device__ __forceinline__ void moments_pair(const OptScalars& s, float clip, float2 g, float2& m, float2& v) {
-  const float2 zero = both(s.minus_zero);
-  g = mul2(g, both(clip));
-  m = add2(fma2(both(s.beta1), m, zero), fma2(both(s.one_minus_beta1), g, zero));
-  v = add2(fma2(both(s.beta2), v, zero), fma2(both(s.one_minus_beta2), mul2(g, g), zero));
-}
-
-__device__ __forceinline__ float2 param_pair(const OptScalars& s, const OptCoefs& c, float2 p, float2 m, float2 v) {
-  const float2 d = fma2(make_float2(sqrt_approx(v.x), sqrt_approx(v.y)), both(c.root), both(s.eps));
-  return fma2(both(-c.rate), mul2(m, make_float2(rcp_approx(d.x), rcp_approx(d.y))), mul2(p, both(c.decay)));
-}
-
-// The approximate root takes subnormal second moments as zero: roots below 2^-63, which with b2 = 0.999 are
-// at most 2^-58 in the denominator and nothing beside an eps from here on.  Below it the step is taken with
-// IEEE root and division, one element at a time.
-constexpr float kLeastEps = 0x1p-33f;
-
-__device__ __forceinline__ void adamw_eight(const OptScalars& s, const OptCoefs& c, float2* p, const float2* g, float2* m, float2* v) {
-  if (s.eps >= kLeastEps) {
-#pragma unroll
-    for (int j = 0; j < 4; j++) {
-      moments_pair(s, c.clip, g[j], m[j], v[j]);
-      p[j] = param_pair(s, c, p[j], m[j], v[j]);
-    }
-  } else {
-    float *ps = reinterpret_cast<float*>(p), *ms = reinterpret_cast<float*>(m), *vs = reinterpret_cast<float*>(v);
-    const float* gs = reinterpret_cast<const float*>(g);
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      opt_moments(s, __fmul_rn(gs[j], c.clip), ms[j], vs[j]);
-      ps[j] = ps[j] * c.decay - c.rate * (ms[j] / (sqrtf(vs[j]) * c.root + s.eps));
-    }
   }
 }
 
@@ -515,106 +463,10 @@ __global__ void __launch_bounds__(kAdamw8Threads, sizeof(P) == 4 || sizeof(G) ==
   opt_advance(b.s, co.t);
 }
 
-// ---- AdamW on a decoder with unit rows --------------------------------------------------------------------
-struct RowArgs {
-  OptScalars s;
-  OptTensor t;
-  long long rows;
-  int cols;
-};
-
-// Sums of two values over the CTA.  `part` is not written again before every thread has passed another barrier.
-__device__ __forceinline__ float2 cta_sum2(float a, float b, float2* part, int warps) {
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, m);
-    b += __shfl_xor_sync(0xffffffffu, b, m);
-  }
-  if (warps == 1) return make_float2(a, b);
-  const int lane = threadIdx.x & 31;
-  if (lane == 0) part[threadIdx.x >> 5] = make_float2(a, b);
-  __syncthreads();
-  const float2 q = lane < warps ? part[lane] : make_float2(0.0f, 0.0f);
-  a = q.x, b = q.y;
-#pragma unroll
-  for (int m = 16; m > 0; m >>= 1) {
-    a += __shfl_xor_sync(0xffffffffu, a, m);
-    b += __shfl_xor_sync(0xffffffffu, b, m);
-  }
-  return make_float2(a, b);
-}
-
-// A team of warps per row at a time, eight elements per thread, so the row stays in registers between the
-// projection, the step and the division by its length.  The team is the CTA, or one of its warps where a warp is
-// enough for a row (rows of up to 256 elements; those need no barrier).
-// MOST: threads of a CTA at most.  Rows of up to 2304 elements (288 threads) are better off with four CTAs on an SM than
-// with the registers of three (65536 rows of 2304 bf16: 541 and 556 us); a fifth would spill (767 us).
-template <typename P, typename G, bool MASTER, int MOST>
-__global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
-  using W = typename std::conditional<MASTER, float, P>::type;
-  __shared__ float2 part[2][32];
-  const bool one_warp = a.cols <= kOptBlock;
-  const int teams = one_warp ? blockDim.x >> 5 : 1, lanes = one_warp ? 32 : blockDim.x, warps = lanes >> 5;
-  const int lane = one_warp ? threadIdx.x & 31 : threadIdx.x;
-  const OptTensor& t = a.t;
-  opt_wait();
-  OptCoefs co;
-  if (!opt_coefs(a.s, co)) return;
-  OptCoefs unclipped = co;                            // the gradient is clipped before the projection
-  unclipped.clip = 1.0f;
-  const long long stride = (long long)gridDim.x * teams;
-  for (long long r = (long long)blockIdx.x * teams + (one_warp ? threadIdx.x >> 5 : 0); r < a.rows; r += stride) {
-    const long long e0 = r * a.cols, end = e0 + a.cols;
-    const bool vec = t.vec && lane * 8 < a.cols;      // the last lanes of an aligned row may have nothing
-    float2 p2[4], g2[4], m2[4], v2[4];
-    float *p = reinterpret_cast<float*>(p2), *g = reinterpret_cast<float*>(g2);
-    if (t.vec && !vec) {
-#pragma unroll
-      for (int j = 0; j < 4; j++) p2[j] = g2[j] = m2[j] = v2[j] = make_float2(0.0f, 0.0f);
-    } else {
-      opt_load<W>(MASTER ? t.master : t.param, e0, end, vec, lane, lanes, p2);
-      opt_load<G>(t.grad, e0, end, vec, lane, lanes, g2);
-      opt_load<float>(t.exp_avg, e0, end, vec, lane, lanes, m2);
-      opt_load<float>(t.exp_avg_sq, e0, end, vec, lane, lanes, v2);
-    }
-    float gp = 0.0f, pp = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) {
-      g[j] *= co.clip;
-      gp = fmaf(g[j], p[j], gp);
-      pp = fmaf(p[j], p[j], pp);
-    }
-    const float2 dots = cta_sum2(gp, pp, part[0], warps);
-    const float along = dots.y > 0.0f ? dots.x / dots.y : 0.0f;
-    float len = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) g[j] -= along * p[j];
-    adamw_eight(a.s, unclipped, p2, g2, m2, v2);
-#pragma unroll
-    for (int j = 0; j < 8; j++) len = fmaf(p[j], p[j], len);
-    len = cta_sum2(len, 0.0f, part[1], warps).x;
-    const float scale = len > 0.0f ? 1.0f / sqrtf(len) : 1.0f;      // a row of zeros stays one
-#pragma unroll
-    for (int j = 0; j < 8; j++) p[j] *= scale;
-    if (t.vec && !vec) continue;
-    opt_store<P>(t.param, e0, end, vec, lane, lanes, p2);
-    if (MASTER) opt_store<float>(t.master, e0, end, vec, lane, lanes, p2);
-    opt_store<float>(t.exp_avg, e0, end, vec, lane, lanes, m2);
-    opt_store<float>(t.exp_avg_sq, e0, end, vec, lane, lanes, v2);
-  }
-  opt_advance(a.s, co.t);
-}
-
 // ---- host side ---------------------------------------------------------------------------------------------
-static size_t opt_size(int dt) { return dt == FLEXSAE_F32 ? 4 : 2; }
-static bool opt_dtype(int dt) { return dt == FLEXSAE_F32 || dt == FLEXSAE_BF16 || dt == FLEXSAE_F16; }
-static bool aligned(const void* p, size_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
-
 constexpr int64_t kOptMaxTensors = 1 << 16;
 constexpr int64_t kOptMaxNumel = 1ll << 38;
 constexpr unsigned long long kOptMaxChunks = 1ull << 30;
-constexpr int kOptSms = 148;
-
 // A stretch of memory that a step reads or writes.
 struct Stretch {
   uintptr_t begin, end;
@@ -717,75 +569,6 @@ static int check_tensors(const flexsae_optim_tensor* t, int64_t n, int state_bit
   return rc;
 }
 
-static OptTensor make_tensor(const flexsae_optim_tensor& t, int64_t i, int state_bits) {
-  OptTensor d;
-  d.param = t.param;
-  d.grad = t.grad;
-  d.exp_avg = t.exp_avg;
-  d.exp_avg_sq = t.exp_avg_sq;
-  d.exp_avg_scale = t.exp_avg_scale;
-  d.exp_avg_sq_scale = t.exp_avg_sq_scale;
-  d.master = t.master;
-  d.numel = t.numel;
-  d.index = (int)i;
-  const size_t state = state_bits == 8 ? 8 : 32;
-  d.vec = aligned(t.param, 8 * opt_size(t.param_dtype)) && aligned(t.grad, 8 * opt_size(t.grad_dtype)) && aligned(t.master, 32) &&
-          aligned(t.exp_avg, state) && aligned(t.exp_avg_sq, state);
-  return d;
-}
-
-// Kernels are compiled per (parameter type, gradient type, master copy): 0 fp32; then bf16 and fp16,
-// each with gradients of its own type or fp32, without and with a master copy.
-constexpr int kOptKinds = 9;
-static int kind_of(const flexsae_optim_tensor& t) {
-  if (t.param_dtype == FLEXSAE_F32) return 0;
-  return 1 + (t.param_dtype == FLEXSAE_F16 ? 4 : 0) + (t.grad_dtype == FLEXSAE_F32 ? 2 : 0) + (t.master ? 1 : 0);
-}
-
-// CTAs of `threads` that the GPU holds at the same time, at most `most` per SM: the grid of a launch whose CTAs take
-// every gridDim-th chunk, so that all of them run from the start and finish together.  Asked for once (`known`).
-template <typename K>
-static cudaError_t resident_ctas(std::atomic<unsigned>& known, K kernel, int threads, int most, unsigned* ctas) {
-  *ctas = known.load(std::memory_order_relaxed);
-  if (*ctas) return cudaSuccess;
-  int n = 0;
-  if (cudaError_t e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, threads, 0)) return e;
-  *ctas = (unsigned)(std::max(1, std::min(n, most)) * kOptSms);
-  known.store(*ctas, std::memory_order_relaxed);
-  return cudaSuccess;
-}
-
-// A launch that is set up while the kernel before it in the stream finishes; every kernel launched so waits for that
-// one (opt_wait) before it touches memory.  4096 unit rows of 256 take 5.5 instead of 8.2 us in a row of such
-// steps, a model of 20 ragged tensors 43.7 instead of 46.  Letting the next kernel in any earlier (from the start of
-// this one) costs more than it gains: 6.4 and 45.4 us.
-template <typename Args>
-static cudaError_t launch_early(void (*kernel)(Args), unsigned grid, int threads, const Args& args, cudaStream_t st) {
-  cudaLaunchAttribute early;
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(grid);
-  config.blockDim = dim3(threads);
-  config.stream = st;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  return cudaLaunchKernelEx(&config, kernel, args);
-}
-
-#define FLEXSAE_OPT_KINDS(kind, CALL)                         \
-  switch (kind) {                                             \
-    case 0: CALL(float, float, false); break;                 \
-    case 1: CALL(__nv_bfloat16, __nv_bfloat16, false); break; \
-    case 2: CALL(__nv_bfloat16, __nv_bfloat16, true); break;  \
-    case 3: CALL(__nv_bfloat16, float, false); break;         \
-    case 4: CALL(__nv_bfloat16, float, true); break;          \
-    case 5: CALL(__half, __half, false); break;               \
-    case 6: CALL(__half, __half, true); break;                \
-    case 7: CALL(__half, float, false); break;                \
-    default: CALL(__half, float, true); break;                \
-  }
-
 // What the loads of one SM have under way at most in the 32-bit step, which sets how many CTAs it is given.
 // More costs HBM throughput: 302 M bf16 parameters take 1.10 / 1.03 / 1.08 ms with 3 / 4 / 5 CTAs of 12 KB
 // each, 268 M fp32 parameters 1.25 / 1.12 / 1.18 ms with 2 / 3 / 4 of 16 KB.
@@ -868,27 +651,6 @@ static int adamw_impl(const flexsae_optim_tensor* t, int64_t n, int state_bits, 
   if (ids != few) delete[] ids;
   if (e != cudaSuccess) return fail((int)e, "AdamW launch failed: %s", cudaGetErrorString(e));
   return 0;
-}
-
-constexpr int kRowTeams = 4;      // warps of a CTA where each has a row of its own
-
-static cudaError_t launch_rows(const RowArgs& a, int kind, cudaStream_t st) {
-  const int row_warps = (a.cols + kOptBlock - 1) / kOptBlock;
-  const int teams = row_warps == 1 ? kRowTeams : 1, warps = row_warps * teams;
-  const long long ctas = (a.rows + teams - 1) / teams;
-  cudaError_t e = cudaSuccess;
-  unsigned most = 0;
-#define CALL_ROWS(P, G, M)                                                                                         \
-  {                                                                                                                \
-    const auto kernel = warps <= 9 ? adamw_unit_rows_kernel<P, G, M, 288> : adamw_unit_rows_kernel<P, G, M, 1024>; \
-    static std::atomic<unsigned> known[33];                                                                        \
-    e = resident_ctas(known[warps], kernel, warps * 32, 32, &most);                                                \
-    if (e == cudaSuccess) e = launch_early(kernel, (unsigned)std::min<long long>(ctas, most), warps * 32, a, st);  \
-  }
-  FLEXSAE_OPT_KINDS(kind, CALL_ROWS)
-#undef CALL_ROWS
-  t_launches++;
-  return e;
 }
 
 template <int N>
@@ -1016,7 +778,6 @@ int flexsae_adamw_unit_rows_step(const flexsae_optim_tensor* tensors_host, int64
     a.s = s;
     a.s.advance = i == last;
     a.t = make_tensor(t, i, 32);
-    a.t.vec = a.t.vec && t.cols % 8 == 0;
     a.rows = t.numel / t.cols;
     a.cols = (int)t.cols;
     if (cudaError_t e = launch_rows(a, kind_of(t), st)) return fail((int)e, "unit-row AdamW launch failed: %s", cudaGetErrorString(e));
