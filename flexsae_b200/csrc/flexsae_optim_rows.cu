@@ -89,8 +89,26 @@ __device__ __forceinline__ float2 team_sum2(float a, float b, float2* part, int 
   return make_float2(a, b);
 }
 
+// What a thread of whole rows reads, as it lies in memory.
+template <typename W, typename G>
+struct RowRaw {
+  Raw8<W> p;
+  Raw8<G> g;
+  Raw8<float> m, v;
+
+  __device__ __forceinline__ void load(const OptTensor& t, bool master, long long first) {
+    p.load(reinterpret_cast<const W*>(master ? t.master : t.param) + first);
+    g.load(reinterpret_cast<const G*>(t.grad) + first);
+    m.load(reinterpret_cast<const float*>(t.exp_avg) + first);
+    v.load(reinterpret_cast<const float*>(t.exp_avg_sq) + first);
+  }
+};
+
 // MOST: threads of a CTA at most.  The registers of a thread (56) are set so that an SM holds four CTAs of up to 288 threads
-// or two of up to 576: rows of up to 2304 elements take 541 us with four CTAs and 556 with three (a fifth spills: 767 us).
+// or two of up to 576: 65536 rows of 2304 bf16 take 541 us with four CTAs and 556 with three (a fifth spills: 767 us).
+// Where an SM holds one CTA, nothing covers its waits, so whole rows of up to 704 threads (88 registers), with 16-bit
+// parameters and gradients up to 896 (72), have the next row's loads under way: 60 M bf16 in rows of 5120 / 7168 take 215 /
+// 206 us with them and 297 / 262 without; fp32 in rows of 7168 would spill (353 and 295).
 template <RowMode MODE, typename P, typename G, bool MASTER, int MOST>
 __global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
   using W = typename std::conditional<MASTER, float, P>::type;      // type that holds the parameter's value
@@ -102,15 +120,23 @@ __global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) a
   if (!opt_coefs(a.s, co)) return;
   OptCoefs unclipped = co;                            // the gradient is clipped before the projection
   unclipped.clip = 1.0f;
+  constexpr bool kAhead = MOST == 704 || MOST == 896;
+  RowRaw<W, G> next = {};
+  if (kAhead && lane * 8 < a.cols && blockIdx.x < a.rows) next.load(t, MASTER, (long long)blockIdx.x * a.cols + lane * 8);
   for (long long r0 = (long long)blockIdx.x * teams; r0 < a.rows; r0 += (long long)gridDim.x * teams) {
     const long long r = r0 + slot, begin = r * a.cols;
     const int n = r < a.rows ? a.cols : 0;            // past the last row a team only keeps its warp company
     float2 p2[4], g2[4], m2[4], v2[4];
     float *p = reinterpret_cast<float*>(p2), *g = reinterpret_cast<float*>(g2);
-    row_load<MODE, W>(MASTER ? t.master : t.param, begin, n, lane, team, p2);
-    row_load<MODE, G>(t.grad, begin, n, lane, team, g2);
-    row_load<MODE, float>(t.exp_avg, begin, n, lane, team, m2);
-    row_load<MODE, float>(t.exp_avg_sq, begin, n, lane, team, v2);
+    if (kAhead) {
+      next.p.pairs(p2), next.g.pairs(g2), next.m.pairs(m2), next.v.pairs(v2);
+      if (lane * 8 < a.cols && r0 + gridDim.x < a.rows) next.load(t, MASTER, begin + (long long)gridDim.x * a.cols + lane * 8);
+    } else {
+      row_load<MODE, W>(MASTER ? t.master : t.param, begin, n, lane, team, p2);
+      row_load<MODE, G>(t.grad, begin, n, lane, team, g2);
+      row_load<MODE, float>(t.exp_avg, begin, n, lane, team, m2);
+      row_load<MODE, float>(t.exp_avg_sq, begin, n, lane, team, v2);
+    }
     float gp = 0.0f, pp = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -139,15 +165,20 @@ __global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) a
 }
 
 constexpr int kRowThreads = 128;      // of a CTA whose rows have a warp or less each
-#ifndef GROUPED
-#define GROUPED 640
-#endif
+// Rows that do not begin at a group of eight are read in groups from here on (their ends are accesses of
+// single elements; bf16: 77220 rows of 777 take 286 us in groups and 325 strided, 131072 of 257 311 and 271).
+constexpr int kGroupedFrom = 640;
 
 template <RowMode MODE, typename P, typename G, bool M>
 static cudaError_t launch_mode(const RowArgs& a, int threads, cudaStream_t st) {
-  const auto kernel = threads <= 288   ? adamw_unit_rows_kernel<MODE, P, G, M, 288>
-                      : threads <= 576 ? adamw_unit_rows_kernel<MODE, P, G, M, 576>
-                                       : adamw_unit_rows_kernel<MODE, P, G, M, 1024>;
+  auto kernel = threads <= 288   ? adamw_unit_rows_kernel<MODE, P, G, M, 288>
+                : threads <= 576 ? adamw_unit_rows_kernel<MODE, P, G, M, 576>
+                                 : adamw_unit_rows_kernel<MODE, P, G, M, 1024>;
+  if constexpr (MODE == kWholeRows) {
+    if (threads > 576 && threads <= 704) kernel = adamw_unit_rows_kernel<MODE, P, G, M, 704>;
+    if constexpr (sizeof(P) == 2 && sizeof(G) == 2 && !M)
+      if (threads > 704 && threads <= 896) kernel = adamw_unit_rows_kernel<MODE, P, G, M, 896>;
+  }
   static std::atomic<unsigned> known[33];
   unsigned most = 0;
   if (cudaError_t e = resident_ctas(known[threads / 32], kernel, threads, 32, &most)) return e;
@@ -160,7 +191,7 @@ cudaError_t launch_rows(RowArgs a, int kind, cudaStream_t st) {
   RowMode mode = kStridedRows;
   if (a.t.vec && a.cols % 8 == 0) {
     mode = kWholeRows;
-  } else if (a.t.vec && a.cols >= GROUPED && (a.cols + 14) / 8 <= 1024) {
+  } else if (a.t.vec && a.cols >= kGroupedFrom && (a.cols + 14) / 8 <= 1024) {
     mode = kGroupedRows;
     groups = (a.cols + 14) / 8;       // one more, since a row may begin inside a group
   }

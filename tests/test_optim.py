@@ -725,7 +725,9 @@ def rows_bounds(b, want, t, lr, clip, betas=(0.9, 0.999), eps=1e-8, decay=0.01):
 
 @gpu
 @pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
-@pytest.mark.parametrize("F,D,offset", [(1, 1, 0), (5, 7, 0), (300, 8, 0), (33, 255, 0), (33, 256, 0), (33, 257, 1), (40, 512, 1), (500, 768, 0), (9, 2304, 0), (3, 8191, 0), (4, 8192, 0)])
+@pytest.mark.parametrize("F,D,offset", [(1, 1, 0), (5, 7, 0), (300, 8, 0), (33, 255, 0), (33, 256, 0), (33, 257, 1), (40, 512, 1), (500, 768, 0), (9, 2304, 0), (3, 8191, 0), (4, 8192, 0),
+                                        (500, 3, 0), (777, 5, 1), (130, 16, 0), (65, 40, 0), (70, 100, 0), (300, 641, 0), (601, 777, 0), (20, 2301, 1),
+                                        (310, 4095, 0), (305, 4616, 0), (300, 5632, 0), (301, 5640, 0), (299, 7168, 0), (5, 7176, 0), (4, 8185, 0), (4, 8186, 0)])
 def test_unit_rows_against_the_oracle(dtype, grad_dtype, master, F, D, offset):
     x = make((F, D), dtype, F + D, master, grad_dtype, offset, spread=False)
     w = x[4] if master else x[0]
