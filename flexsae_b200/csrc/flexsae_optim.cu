@@ -21,7 +21,9 @@ namespace flexsae {
 constexpr int kNormUnits = 4;                               // units of 256 elements a warp takes at a time
 constexpr int kNormGrid = 148 * 8;
 constexpr int kNormCluster = 8, kNormClusterThreads = 512;
-constexpr int64_t kNormSmall = 1 << 19;                     // elements of a list for which one cluster is enough: four rounds
+// Elements of a list for which one cluster is enough.  With 2^17 / 2^18 / 2^19 it takes 2.7 / 3.3 / 4.6 us and two launches 3.0 on
+// the GPU, but 4.7 and 7.8 us where the host has to keep up.
+constexpr int64_t kNormSmall = 1 << 18;
 // Tensors of one launch.  What a launch's arguments hold is paid for on the host: a step over 20 tensors takes the
 // caller 14 us with room for 32 of them and 23 us with room for 256; the GPU does not notice (3.2 us either way).
 constexpr int kSmallBatch = 32, kLargeBatch = 256;

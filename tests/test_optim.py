@@ -173,10 +173,10 @@ def test_norm_entry_refuses_before_any_launch():
     assert lib.flexsae_grad_norm_workspace_bytes(1 << 17, 8, ctypes.byref(size)) == -1
     assert lib.flexsae_grad_norm_workspace_bytes(2, -1, ctypes.byref(size)) == -1
     assert lib.flexsae_grad_norm_workspace_bytes(2, 8, None) == -1
-    assert workspace(32, 1 << 19) == 0                            # one cluster, no scratch memory
+    assert workspace(32, 1 << 18) == 0                            # one cluster, no scratch memory
     large = 1 << 20
     need = workspace(2, large)
-    assert need > 0 and workspace(33, 8) > 0 and workspace(32, (1 << 19) + 1) > 0
+    assert need > 0 and workspace(33, 8) > 0 and workspace(32, (1 << 18) + 1) > 0
 
     def call(grads=(64, 1 << 30), numel=(large, 4), dtypes=(0, 1), n=2, out=512, ws=1024, ws_bytes=need):
         return lib.flexsae_grad_norm((ctypes.c_void_p * 2)(*grads), (ctypes.c_int64 * 2)(*numel), (ctypes.c_int32 * 2)(*dtypes), n, out, ws,
@@ -281,7 +281,7 @@ NORM_TOL = 5 * U
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
-@pytest.mark.parametrize("n,offset", [(1, 0), (7, 0), (255, 1), (256, 0), (257, 3), (8191, 0), (8192, 0), (8193, 1), (100003, 0), (1 << 19, 0), ((1 << 19) + 1, 0), (20_000_001, 0)])
+@pytest.mark.parametrize("n,offset", [(1, 0), (7, 0), (255, 1), (256, 0), (257, 3), (8191, 0), (8192, 0), (8193, 1), (100003, 0), (1 << 18, 0), ((1 << 18) + 1, 0), (20_000_001, 0)])
 def test_norm_of_one_tensor(dtype, n, offset):
     x = torch.randn(n + offset, generator=torch.Generator().manual_seed(n)).to(dtype).cuda()[offset:]
     want = float(x.double().square().sum().sqrt())
