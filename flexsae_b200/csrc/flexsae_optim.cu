@@ -270,6 +270,15 @@ __device__ __forceinline__ float max_abs3(float a, float b, float c) {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= FLT_MAX; }
 
+// (x << SHIFT) + y.  Written as instructions: with both summands shifted in C++, the compiler (12.9) dropped the shift in
+// one arrangement of the code that follows.
+template <int SHIFT>
+__device__ __forceinline__ unsigned shift_add(unsigned x, unsigned y) {
+  unsigned d;
+  asm("{.reg .b32 t; shl.b32 t, %1, %2; add.u32 %0, t, %3;}" : "=r"(d) : "r"(x), "n"(SHIFT), "r"(y));
+  return d;
+}
+
 // Top bytes of four words, lowest first.
 __device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
@@ -435,14 +444,16 @@ struct Adamw8Step {
       const float2 yv = mul2(mul2(v[j], iv), both(0x1p-112f));
       const unsigned m0 = __float_as_uint(ym.x), m1 = __float_as_uint(ym.y);
       const unsigned v0 = __float_as_uint(fmaxf(yv.x, __uint_as_float(kLeastV))), v1 = __float_as_uint(fmaxf(yv.y, __uint_as_float(kLeastV)));
-      qm[2 * j] = ((m0 << 4) + (h >> 8)) | (m0 & 0x80000000u);
-      qm[2 * j + 1] = ((m1 << 4) + (h << 4 & 0xffffffu)) | (m1 & 0x80000000u);
-      qv[2 * j] = (v0 << 3) + (h << 3 & 0xffffffu);
-      qv[2 * j + 1] = (v1 << 3) + (h >> 8);
+      qm[2 * j] = shift_add<4>(m0, h >> 8) | (m0 & 0x80000000u);
+      qm[2 * j + 1] = shift_add<4>(m1, h << 4 & 0xffffffu) | (m1 & 0x80000000u);
+      qv[2 * j] = shift_add<3>(v0, h << 3 & 0xffffffu);
+      qv[2 * j + 1] = shift_add<3>(v1, h >> 8);
     }
     Raw8<unsigned char> cm, cv;
     cm.w = make_uint2(top_bytes(qm[0], qm[1], qm[2], qm[3]), top_bytes(qm[4], qm[5], qm[6], qm[7]));
     cv.w = make_uint2(top_bytes(qv[0], qv[1], qv[2], qv[3]), top_bytes(qv[4], qv[5], qv[6], qv[7]));
+    // The floor of v (see code_e5m2) on the finished codes, four at a time: 0 becomes 1, since a byte of at most 0x7f has
+    // its top bit set after 0x7f was added unless it is 0.
     cm.store(at.m + e);
     cv.store(at.v + e);
     if (threadIdx.x % 32 == 0) {

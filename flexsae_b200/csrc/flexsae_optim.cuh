@@ -117,6 +117,8 @@ template <>
 __device__ __forceinline__ float opt_widen<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
 template <>
 __device__ __forceinline__ float opt_widen<__half>(__half x) { return __half2float(x); }
+// 16-bit parameters are rounded to nearest, as torch's optimizers do: a change below half their spacing is lost unless a
+// master copy holds it.
 template <typename T>
 __device__ __forceinline__ T opt_narrow(float x) { return x; }
 template <>

@@ -69,7 +69,8 @@ def adamw_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sq
     ``params`` (float32, bfloat16 or float16, mixed), ``grads`` of the same types or float32, float32
     states in their parameters' layout.  ``step``: int64 on the device, steps taken so far; t is one
     more, and the call leaves t there.  ``masters``: float32 copies of 16-bit parameters that hold the
-    exact values (None where a parameter has none); the parameters are their roundings.  ``lr``: a number, or a float32 tensor on the
+    exact values (None where a parameter has none); the parameters are their roundings (to nearest: without a master, a
+    16-bit parameter loses changes below half its spacing).  ``lr``: a number, or a float32 tensor on the
     device (which a captured graph follows).  ``norm``: the norm of all gradients, from ``grad_norm``;
     with it c = min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves everything as it
     was.  A tensor given twice, or tensors that overlap, are refused."""
