@@ -369,6 +369,19 @@ def test_adamw_on_many_tensors_of_all_kinds_with_empty_ones():
 
 
 @gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
+def test_adamw_long_lists_of_every_kind(dtype, grad_dtype, master):
+    sets = [make((1024 * (k % 3) + 40 * k + 1,), dtype, 300 + k, master, grad_dtype) for k in range(40)]
+    before = [[f64(x[4] if master else x[0]), f64(x[1]), f64(x[2]), f64(x[3])] for x in sets]
+    optim.adamw_step(*[[x[k] for x in sets] for k in range(4)], steps_in(6), lr=1e-3, masters=[x[4] for x in sets])
+    for x, b in zip(sets, before):
+        want = orc.adamw(*b, 7, 1e-3)
+        ep, em, ev = bounds(b, want, 7, 1e-3, (0.9, 0.999), 1e-8, 1.0)
+        check_params(x[0], x[4], want[0], ep, dtype)
+        close(x[2], want[1], em, "m"), close(x[3], want[2], ev, "v")
+
+
+@gpu
 def test_only_empty_tensors_still_count_the_step():
     e, step = [torch.empty(0, device="cuda") for _ in range(4)], steps_in(7)
     optim.adamw_step(*[[x] for x in e], step, lr=1e-3)
@@ -521,6 +534,22 @@ def test_adamw8_states_are_the_oracles_bits(dtype, master, offset, clipped):
             rate, denom = 2e-3 / (1 - 0.9 ** t), np.sqrt(v) / math.sqrt(1 - 0.999 ** t) + 1e-6
             want = p * (1 - 2e-3 * 0.01) - rate * m / denom
             check_params(x[0], x[6], want, 4 * U * np.abs(p) + 32 * U * rate * np.abs(m) / denom, dtype)
+
+
+@gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
+@pytest.mark.parametrize("count", [2, 40])
+def test_adamw8_every_compiled_kernel_rounds_alike(dtype, grad_dtype, master, count):
+    """The kernels are compiled for every combination of types and for short and long lists: each of them bit for bit."""
+    sets = [make8((4096 + 77,), dtype, 90 + k, master) for k in range(count)]
+    for x in sets:
+        x[1] = x[1].to(grad_dtype)
+    before = [[x[1].float().cpu().numpy(), bytes_of(x[2]), x[3].cpu().numpy(), bytes_of(x[4]), x[5].cpu().numpy()] for x in sets]
+    optim.adamw8_step(*[[x[j] for x in sets] for j in range(6)], steps_in(6), lr=2e-3, masters=[x[6] for x in sets], seed=2 ** 32 - 1)
+    for i, (x, b) in enumerate(zip(sets, before)):
+        _, _, m8, ms, v8, vs = orc.adamw8_states(*b, 7, 2 ** 32 - 1, i)
+        assert np.array_equal(x[3].cpu().numpy(), ms) and np.array_equal(x[5].cpu().numpy(), vs)
+        assert np.array_equal(bytes_of(x[2]), m8) and np.array_equal(bytes_of(x[4]), v8)
 
 
 @gpu
