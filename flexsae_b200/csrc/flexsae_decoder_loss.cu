@@ -403,7 +403,7 @@ using namespace flexsae;
 
 extern "C" {
 
-int flexsae_version(void) { return 300; }
+int flexsae_version(void) { return 400; }
 
 const char* flexsae_last_error(void) { return t_err; }
 
