@@ -115,7 +115,9 @@ class AdamW(torch.optim.Optimizer):
     ``norm`` holds the norm of the last step (a 0-dim tensor on the device).
 
     A parameter without a gradient is passed over; its own step count does not move.  All parameters
-    live on one device."""
+    live on one device.  A parameter with a master copy is its rounding after every step: who changes one
+    changes both.  A step may be captured in a CUDA graph once every parameter has its states, that is
+    after a step outside of it (a capture that would have to make them is refused)."""
 
     def __init__(self, params: Iterable, lr: Union[float, torch.Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
                  eps: float = 1e-8, weight_decay: float = 0.01, *, state_bits: int = 32, master_weights: bool = False,
@@ -133,6 +135,8 @@ class AdamW(torch.optim.Optimizer):
         try:
             if group["state_bits"] not in (8, 32):
                 raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+            if not 0 <= group["seed"] < 2 ** 32:
+                raise ValueError(f"seed must be in [0, 2**32), got {group['seed']}")
             if group["unit_rows"] and group["state_bits"] != 32:
                 raise ValueError("unit_rows goes with 32-bit states")
             for p in group["params"]:
@@ -159,7 +163,10 @@ class AdamW(torch.optim.Optimizer):
         """The group's parameters with gradients, those that share a step count together."""
         active = [p for p in group["params"] if p.grad is not None]
         new = [p for p in active if not self.state[p]]
+        capturing = active and active[0].is_cuda and torch.cuda.is_current_stream_capturing()
         if new:
+            if capturing:      # every replay would set them back to zero
+                raise RuntimeError("the optimizer's states have to exist before a step is captured: take one step outside of the graph")
             step = torch.zeros((), dtype=torch.int64, device=new[0].device)
             for p in new:
                 self.state[p].update(self._new_state(p, group, step))
@@ -167,6 +174,8 @@ class AdamW(torch.optim.Optimizer):
             moving = {id(self.state[p]["step"]) for p in active}
             for p in group["params"]:
                 if p.grad is None and self.state.get(p) and id(self.state[p]["step"]) in moving:
+                    if capturing:      # every replay would copy the count again
+                        raise RuntimeError("a parameter that takes part in steps outside of the captured one has no gradient in it")
                     self.state[p]["step"] = self.state[p]["step"].clone()
         counts: Dict[int, List[torch.Tensor]] = {}
         for p in active:
@@ -184,12 +193,12 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for group in self.param_groups for p in group["params"] if p.grad is not None]
             if grads:
                 self.norm = grad_norm(grads)
-        for group in self.param_groups:
+        for index, group in enumerate(self.param_groups):
             for ps in self._cohorts(group):
-                self._step_cohort(group, ps)
+                self._step_cohort(index, group, ps)
         return loss
 
-    def _step_cohort(self, group: dict, ps: List[torch.Tensor]) -> None:
+    def _step_cohort(self, index: int, group: dict, ps: List[torch.Tensor]) -> None:
         states = [self.state[p] for p in ps]
 
         def column(name: str) -> List[Optional[torch.Tensor]]:
@@ -199,8 +208,9 @@ class AdamW(torch.optim.Optimizer):
         kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                   masters=masters if any(t is not None for t in masters) else None, norm=self.norm, max_norm=self.max_norm)
         if group["state_bits"] == 8:
+            seed = (group["seed"] + 0x9E3779B9 * index) % 2 ** 32      # groups of one seed round independently
             adamw8_step(ps, grads, column("exp_avg"), column("exp_avg_scale"), column("exp_avg_sq"), column("exp_avg_sq_scale"),
-                        states[0]["step"], seed=group["seed"], **kw)
+                        states[0]["step"], seed=seed, **kw)
         else:
             step = adamw_unit_rows_step if group["unit_rows"] else adamw_step
             step(ps, grads, column("exp_avg"), column("exp_avg_sq"), states[0]["step"], **kw)
@@ -231,6 +241,8 @@ class AdamW(torch.optim.Optimizer):
                     dtype = torch.float32 if group["state_bits"] == 32 else value.dtype
                     kept = torch.empty_like(p, dtype=dtype, memory_format=torch.preserve_format)
                     self.state[p][name] = kept.copy_(value)
+            if self.state.get(p) and group["master_weights"] and p.dtype != torch.float32 and "master" not in self.state[p]:
+                self.state[p]["master"] = p.detach().to(torch.float32, memory_format=torch.preserve_format)
         for group in self.param_groups:
             counts: Dict[int, torch.Tensor] = {}
             for p in group["params"]:

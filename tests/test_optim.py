@@ -207,7 +207,7 @@ def test_python_entries_need_cuda_tensors():
 
 def test_optimizer_class_refuses_what_it_cannot_do():
     p, q = torch.nn.Parameter(torch.zeros(4, 8)), torch.nn.Parameter(torch.zeros(8))
-    for bad in (dict(state_bits=16), dict(state_bits=8, unit_rows=True), dict(max_norm=0.0), dict(max_norm=-1.0)):
+    for bad in (dict(state_bits=16), dict(state_bits=8, unit_rows=True), dict(max_norm=0.0), dict(max_norm=-1.0), dict(seed=-1), dict(seed=2 ** 32)):
         with pytest.raises(ValueError):
             optim.AdamW([p], **bad)
     with pytest.raises(ValueError, match="unit rows"):
@@ -827,6 +827,55 @@ def test_captured_steps_replay_like_eager_ones(bits):
 
     for a, b in zip(train(False), train(True)):
         assert torch.equal(a, b)
+
+
+@gpu
+def test_a_capture_that_would_make_or_split_states_is_refused():
+    """States made inside a capture would be set to zero by every replay, a step count split there copied by each."""
+    ps = [torch.nn.Parameter(torch.ones(300, device="cuda")) for _ in range(2)]
+    opt = optim.AdamW(ps, lr=1e-2)
+    for p in ps:
+        p.grad = torch.ones_like(p)
+
+    def capture():
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            opt.step()
+        return graph
+
+    with pytest.raises(RuntimeError, match="before a step is captured"):
+        capture()
+    assert not any(opt.state.get(p) for p in ps)
+    opt.step()
+    ps[1].grad = None
+    with pytest.raises(RuntimeError, match="no gradient"):
+        capture()
+    assert opt.state[ps[0]]["step"] is opt.state[ps[1]]["step"]
+    ps[1].grad = torch.ones_like(ps[1])
+    graph = capture()
+    for _ in range(3):
+        graph.replay()
+    assert int(opt.state[ps[0]]["step"]) == 4 and torch.equal(ps[0], ps[1])
+
+
+@gpu
+def test_groups_of_one_seed_round_independently_and_masters_come_with_a_foreign_state():
+    p, q = (torch.nn.Parameter(torch.zeros(1 << 16, device="cuda")) for _ in range(2))
+    opt = optim.AdamW([{"params": [p]}, {"params": [q]}], lr=1e-3, state_bits=8, seed=5)
+    for x in (p, q):
+        x.grad = torch.randn(1 << 16, generator=torch.Generator().manual_seed(0)).cuda()
+    opt.step()
+    same = (opt.state[p]["exp_avg"].view(torch.uint8) == opt.state[q]["exp_avg"].view(torch.uint8)).float().mean()
+    assert torch.equal(p, q) and 0.3 < float(same) < 0.95             # rounded apart: alike with probability q^2 + (1 - q)^2, 2/3 on average
+    a = torch.nn.Parameter(torch.randn(100, device="cuda").bfloat16())
+    a.grad = torch.randn_like(a)
+    theirs, ours = torch.optim.AdamW([a], lr=1e-3), optim.AdamW([a], lr=1e-3, master_weights=True)
+    theirs.step()
+    ours.load_state_dict(theirs.state_dict())
+    assert torch.equal(ours.state[a]["master"], a.detach().float())
+    ours.step()
+    assert torch.equal(ours.state[a]["master"].bfloat16(), a.detach())
 
 
 @gpu
