@@ -220,14 +220,23 @@ class AdamW(torch.optim.Optimizer):
 
     def __setstate__(self, state: dict) -> None:
         super().__setstate__(state)
-        for group in self.param_groups:                 # a state of torch.optim.AdamW knows fewer options
+        for group in self.param_groups:                 # a copy pickled by an earlier version knows fewer options
             for name, value in self.defaults.items():
                 group.setdefault(name, value)
 
+    def _completed(self, state_dict: dict) -> dict:
+        """``state_dict``, its groups with this optimizer's values for the options that they do not have."""
+        saved, mine = state_dict["param_groups"], self.param_groups
+        if len(saved) != len(mine):                     # refused by the base class
+            return state_dict
+        own = [{name: group[name] for name in self.defaults} for group in mine]
+        return {**state_dict, "param_groups": [{**options, **group} for options, group in zip(own, saved)]}
+
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores a ``state_dict``, also one of ``torch.optim.AdamW`` for 32-bit states: the states keep their own types
-        (the base class would turn them into the parameters'), and parameters of a group that stand at the same step
-        share their count again."""
+        (the base class would turn them into the parameters'), parameters of a group that stand at the same step
+        share their count again, and a group keeps its own value of each option that the saved one does not have."""
+        state_dict = self._completed(state_dict)
         super().load_state_dict(state_dict)
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [(p, group) for group in self.param_groups for p in group["params"]]

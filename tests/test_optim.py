@@ -220,6 +220,33 @@ def test_optimizer_class_refuses_what_it_cannot_do():
     assert len(opt.param_groups) == 1                              # a refused group is not kept
 
 
+# ---- CPU: loading states ---------------------------------------------------------------------------------
+def theirs_after_a_step(groups, cls=torch.optim.AdamW, **kw):
+    """A torch optimizer over ``groups`` (lists of parameters) that has taken one step."""
+    opt = cls([{"params": ps} for ps in groups], **{**dict(lr=1e-3), **kw})
+    for ps in groups:
+        for p in ps:
+            p.grad = torch.randn(p.shape, generator=torch.Generator().manual_seed(p.numel())).to(p.dtype)
+    opt.step()
+    return opt
+
+
+def test_options_of_a_group_outlive_a_state_that_does_not_know_them():
+    """torch.optim.AdamW's groups say nothing of unit rows, master copies, seeds: each group keeps its own."""
+    w, b, d = (torch.nn.Parameter(torch.randn(s).to(t)) for s, t in (((6, 8), torch.bfloat16), ((6,), torch.float32), ((6, 8), torch.float32)))
+    theirs = theirs_after_a_step([[w], [b], [d]], lr=7e-3)
+    ours = optim.AdamW([{"params": [w], "master_weights": True}, {"params": [b]}, {"params": [d], "unit_rows": True, "seed": 3}], lr=1e-3, seed=8)
+    ours.load_state_dict(theirs.state_dict())
+    got = [(x["lr"], x["unit_rows"], x["master_weights"], x["seed"], x["state_bits"]) for x in ours.param_groups]
+    assert got == [(7e-3, False, True, 8, 32), (7e-3, False, False, 8, 32), (7e-3, True, False, 3, 32)]
+    assert torch.equal(ours.state[w]["master"], w.detach().float())
+    assert "master" not in ours.state[b] and "master" not in ours.state[d]
+    # a state of its own says all of it, and is followed
+    other = optim.AdamW([{"params": [torch.nn.Parameter(p.detach().clone())]} for p in (w, b, d)], lr=1e-2)
+    other.load_state_dict(ours.state_dict())
+    assert [(x["lr"], x["unit_rows"], x["master_weights"], x["seed"], x["state_bits"]) for x in other.param_groups] == got
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
