@@ -232,11 +232,31 @@ class AdamW(torch.optim.Optimizer):
         own = [{name: group[name] for name in self.defaults} for group in mine]
         return {**state_dict, "param_groups": [{**options, **group} for options, group in zip(own, saved)]}
 
+    @staticmethod
+    def _check_loaded(state_dict: dict) -> None:
+        """Refuses a state that these steps would not continue: of another rule, or without the moments."""
+        for group in state_dict["param_groups"]:
+            for name in ("maximize", "amsgrad"):
+                if group.get(name):
+                    raise ValueError(f"the state was saved with {name}=True, which this optimizer does not have")
+            # torch's Adam family says how the decay is applied; of its members only Adam and AdamW know amsgrad
+            if "momentum_decay" in group or ("decoupled_weight_decay" in group and "amsgrad" not in group):
+                raise ValueError("the state is not one of torch.optim.AdamW: its optimizer follows another rule")
+            if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0) != 0:
+                raise ValueError("the state was saved by an optimizer that adds weight_decay to the gradient (torch.optim.Adam)")
+            for i in group["params"]:
+                state = state_dict["state"].get(i)
+                missing = [name for name in ("step", "exp_avg", "exp_avg_sq") if name not in state] if state else []
+                if missing:
+                    raise ValueError(f"the state of parameter {i} has no {', '.join(missing)}: it is not one of AdamW")
+
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores a ``state_dict``, also one of ``torch.optim.AdamW`` for 32-bit states: the states keep their own types
         (the base class would turn them into the parameters'), parameters of a group that stand at the same step
-        share their count again, and a group keeps its own value of each option that the saved one does not have."""
+        share their count again, and a group keeps its own value of each option that the saved one does not have.  A state
+        of another rule (``maximize``, ``amsgrad``, decay added to the gradient) is refused, with nothing changed."""
         state_dict = self._completed(state_dict)
+        self._check_loaded(state_dict)
         super().load_state_dict(state_dict)
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [(p, group) for group in self.param_groups for p in group["params"]]

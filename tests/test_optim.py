@@ -247,6 +247,26 @@ def test_options_of_a_group_outlive_a_state_that_does_not_know_them():
     assert [(x["lr"], x["unit_rows"], x["master_weights"], x["seed"], x["state_bits"]) for x in other.param_groups] == got
 
 
+@pytest.mark.parametrize("cls,kw,text", [
+    (torch.optim.AdamW, dict(maximize=True), "maximize"), (torch.optim.AdamW, dict(amsgrad=True), "amsgrad"),
+    (torch.optim.Adam, dict(weight_decay=0.1), "weight_decay"), (torch.optim.NAdam, {}, "torch.optim.AdamW"),
+    (torch.optim.RAdam, {}, "torch.optim.AdamW"), (torch.optim.RAdam, dict(decoupled_weight_decay=True), "torch.optim.AdamW"),
+    (torch.optim.SGD, dict(momentum=0.9), "exp_avg"),
+])
+def test_states_of_other_rules_are_refused_before_anything_changes(cls, kw, text):
+    p, q = (torch.nn.Parameter(torch.randn(5, 8)) for _ in range(2))
+    ours = optim.AdamW([{"params": [p]}, {"params": [q]}], lr=2e-3)
+    ours.load_state_dict(theirs_after_a_step([[p], [q]], lr=2e-3).state_dict())
+    kept = {x: dict(ours.state[x]) for x in (p, q)}
+    with pytest.raises(ValueError, match=text):
+        ours.load_state_dict(theirs_after_a_step([[p], [q]], cls, **kw).state_dict())
+    assert all(ours.state[x][name] is value for x in (p, q) for name, value in kept[x].items())
+    assert ours.param_groups[0]["lr"] == 2e-3
+    # without decay Adam is the same rule
+    ours.load_state_dict(theirs_after_a_step([[p], [q]], torch.optim.Adam).state_dict())
+    assert ours.param_groups[0]["lr"] == 1e-3
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
