@@ -233,8 +233,14 @@ class AdamW(torch.optim.Optimizer):
         return {**state_dict, "param_groups": [{**options, **group} for options, group in zip(own, saved)]}
 
     @staticmethod
+    def _check_names(i: int, state: dict, names: Iterable[str]) -> None:
+        missing = [name for name in names if name not in state]
+        if missing:
+            raise ValueError(f"the state of parameter {i} has no {', '.join(missing)}: it is not one of AdamW")
+
+    @staticmethod
     def _check_loaded(state_dict: dict) -> None:
-        """Refuses a state that these steps would not continue: of another rule, or without the moments."""
+        """Refuses a state that these steps would not continue: of another rule, or without the moments in the group's form."""
         for group in state_dict["param_groups"]:
             for name in ("maximize", "amsgrad"):
                 if group.get(name):
@@ -246,15 +252,24 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the state was saved by an optimizer that adds weight_decay to the gradient (torch.optim.Adam)")
             for i in group["params"]:
                 state = state_dict["state"].get(i)
-                missing = [name for name in ("step", "exp_avg", "exp_avg_sq") if name not in state] if state else []
-                if missing:
-                    raise ValueError(f"the state of parameter {i} has no {', '.join(missing)}: it is not one of AdamW")
+                if not state:
+                    continue
+                eight = group.get("state_bits") == 8
+                AdamW._check_names(i, state, ("step", "exp_avg", "exp_avg_sq"))
+                kinds = (state["exp_avg"].dtype, state["exp_avg_sq"].dtype)
+                if eight and kinds != STATE8_DTYPES:
+                    raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 8-bit states takes {STATE8_DTYPES}")
+                if not eight and any(k.itemsize < 2 for k in kinds):
+                    raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 32-bit states takes neither")
+                if eight:
+                    AdamW._check_names(i, state, ("exp_avg_scale", "exp_avg_sq_scale"))
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores a ``state_dict``, also one of ``torch.optim.AdamW`` for 32-bit states: the states keep their own types
         (the base class would turn them into the parameters'), parameters of a group that stand at the same step
         share their count again, and a group keeps its own value of each option that the saved one does not have.  A state
-        of another rule (``maximize``, ``amsgrad``, decay added to the gradient) is refused, with nothing changed."""
+        of another rule (``maximize``, ``amsgrad``, decay added to the gradient), or with moments of other types than ``state_bits`` has, is refused, with
+        nothing changed."""
         state_dict = self._completed(state_dict)
         self._check_loaded(state_dict)
         super().load_state_dict(state_dict)

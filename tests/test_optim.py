@@ -267,6 +267,47 @@ def test_states_of_other_rules_are_refused_before_anything_changes(cls, kw, text
     assert ours.param_groups[0]["lr"] == 1e-3
 
 
+def with_states8(p, seed=0, **kw):
+    """An optimizer with made-up 8-bit states of ``p`` (every scale another), and what they stand for."""
+    opt = optim.AdamW([p], state_bits=8, **kw)
+    state = opt._new_state(p, opt.param_groups[0], torch.tensor(3))
+    g = torch.Generator().manual_seed(seed)
+    for name, top in (("exp_avg", 0x7F), ("exp_avg_sq", 0x7C)):
+        state[name].view(torch.uint8).copy_(torch.randint(1, top, p.shape, generator=g))
+        state[name + "_scale"].copy_(1.0 + torch.arange(optim.state8_blocks(p.numel())))
+    opt.state[p].update(state)
+    return opt
+
+
+def values8(opt, p, name):
+    """What the 8-bit state of ``p`` stands for: its scales go with the elements in memory order."""
+    state = opt.state[p]
+    order = torch.arange(p.numel()).as_strided(p.shape, p.stride())
+    return state[name].float() * state[name + "_scale"][order // 256]
+
+
+def test_float_moments_are_not_loaded_into_8_bit_states_nor_codes_into_32_bit_ones():
+    p = torch.nn.Parameter(torch.randn(5, 8))
+    theirs = theirs_after_a_step([[p]])
+    ours = optim.AdamW([p], state_bits=8)
+    with pytest.raises(TypeError, match="8-bit"):
+        ours.load_state_dict(theirs.state_dict())
+    assert not ours.state
+    eight = with_states8(p).state_dict()
+    ours.load_state_dict(eight)
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert ours.state[p][name].dtype in optim.STATE8_DTYPES and torch.equal(values8(ours, p, name), values8(with_states8(p), p, name))
+    for broken in (dict(state_bits=32), dict(params=[0])):              # a group that says otherwise, or that says nothing
+        groups = [{k: v for k, v in {**eight["param_groups"][0], **broken}.items() if k != "state_bits" or "params" not in broken}]
+        ours = optim.AdamW([p])
+        with pytest.raises(TypeError, match="32-bit"):
+            ours.load_state_dict({**eight, "param_groups": groups})
+        assert not ours.state
+    without = {**eight, "state": {0: {k: v for k, v in eight["state"][0].items() if k != "exp_avg_scale"}}}
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        optim.AdamW([p], state_bits=8).load_state_dict(without)
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
