@@ -42,6 +42,10 @@ def state8_blocks(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
+def _same_layout(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.numel() == 0 or all(n == 1 or s == t for n, s, t in zip(a.shape, a.stride(), b.stride()))
+
+
 def _step(kind: int, params, grads, exp_avgs, scales, exp_avg_sqs, sq_scales, masters, step, lr, betas, eps, weight_decay, norm,
           max_norm, seed=0) -> None:
     _losses.launch_count += nv.binding().step(kind, params, grads, exp_avgs, scales, exp_avg_sqs, sq_scales, masters, step, lr,
@@ -238,10 +242,9 @@ class AdamW(torch.optim.Optimizer):
         if missing:
             raise ValueError(f"the state of parameter {i} has no {', '.join(missing)}: it is not one of AdamW")
 
-    @staticmethod
-    def _check_loaded(state_dict: dict) -> None:
+    def _check_loaded(self, state_dict: dict) -> None:
         """Refuses a state that these steps would not continue: of another rule, or without the moments in the group's form."""
-        for group in state_dict["param_groups"]:
+        for group, mine in zip(state_dict["param_groups"], self.param_groups):
             for name in ("maximize", "amsgrad"):
                 if group.get(name):
                     raise ValueError(f"the state was saved with {name}=True, which this optimizer does not have")
@@ -250,26 +253,29 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError("the state is not one of torch.optim.AdamW: its optimizer follows another rule")
             if not group.get("decoupled_weight_decay", True) and group.get("weight_decay", 0) != 0:
                 raise ValueError("the state was saved by an optimizer that adds weight_decay to the gradient (torch.optim.Adam)")
-            for i in group["params"]:
+            for i, p in zip(group["params"], mine["params"]):
                 state = state_dict["state"].get(i)
                 if not state:
                     continue
                 eight = group.get("state_bits") == 8
-                AdamW._check_names(i, state, ("step", "exp_avg", "exp_avg_sq"))
+                self._check_names(i, state, ("step", "exp_avg", "exp_avg_sq"))
                 kinds = (state["exp_avg"].dtype, state["exp_avg_sq"].dtype)
                 if eight and kinds != STATE8_DTYPES:
                     raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 8-bit states takes {STATE8_DTYPES}")
                 if not eight and any(k.itemsize < 2 for k in kinds):
                     raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 32-bit states takes neither")
                 if eight:
-                    AdamW._check_names(i, state, ("exp_avg_scale", "exp_avg_sq_scale"))
+                    self._check_names(i, state, ("exp_avg_scale", "exp_avg_sq_scale"))
+                    if not (_same_layout(state["exp_avg"], p) and _same_layout(state["exp_avg_sq"], p)):
+                        raise ValueError(f"the 8-bit states of parameter {i} were saved in another memory layout: their scales go with "
+                                         f"256 elements that lie side by side (strides {state['exp_avg'].stride()}, the parameter's {p.stride()})")
 
     def load_state_dict(self, state_dict: dict) -> None:
         """Restores a ``state_dict``, also one of ``torch.optim.AdamW`` for 32-bit states: the states keep their own types
         (the base class would turn them into the parameters'), parameters of a group that stand at the same step
         share their count again, and a group keeps its own value of each option that the saved one does not have.  A state
         of another rule (``maximize``, ``amsgrad``, decay added to the gradient), or with moments of other types than ``state_bits`` has, is refused, with
-        nothing changed."""
+        nothing changed; so are 8-bit states saved from a parameter of another memory layout."""
         state_dict = self._completed(state_dict)
         self._check_loaded(state_dict)
         super().load_state_dict(state_dict)

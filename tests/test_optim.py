@@ -308,6 +308,26 @@ def test_float_moments_are_not_loaded_into_8_bit_states_nor_codes_into_32_bit_on
         optim.AdamW([p], state_bits=8).load_state_dict(without)
 
 
+@pytest.mark.parametrize("shape", [(64, 40), (4, 512)])
+def test_8_bit_states_of_another_layout_are_refused(shape):
+    """A scale belongs to 256 elements that lie side by side: in another order its elements are others."""
+    plain = torch.nn.Parameter(torch.randn(shape))
+    turned = torch.nn.Parameter(torch.randn(shape[::-1]).t())
+    for p, q in ((plain, turned), (turned, plain)):
+        saved = with_states8(p)
+        ours = optim.AdamW([q], state_bits=8)
+        with pytest.raises(ValueError, match="layout"):
+            ours.load_state_dict(saved.state_dict())
+        assert not ours.state
+        ours = optim.AdamW([torch.nn.Parameter(p.detach().clone())], state_bits=8)
+        ours.load_state_dict(saved.state_dict())
+        for name in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(values8(ours, ours.param_groups[0]["params"][0], name), values8(saved, p, name))
+    wide = optim.AdamW([turned])                                       # 32-bit states go by their elements
+    wide.load_state_dict(theirs_after_a_step([[plain]]).state_dict())
+    assert wide.state[turned]["exp_avg"].stride() == turned.stride()
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
