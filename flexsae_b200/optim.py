@@ -259,6 +259,9 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 eight = group.get("state_bits") == 8
                 self._check_names(i, state, ("step", "exp_avg", "exp_avg_sq"))
+                for name in ("exp_avg", "exp_avg_sq", "master"):
+                    if name in state and state[name].shape != p.shape:
+                        raise ValueError(f"{name} of parameter {i} has shape {tuple(state[name].shape)}, the parameter {tuple(p.shape)}")
                 kinds = (state["exp_avg"].dtype, state["exp_avg_sq"].dtype)
                 if eight and kinds != STATE8_DTYPES:
                     raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 8-bit states takes {STATE8_DTYPES}")
@@ -266,6 +269,9 @@ class AdamW(torch.optim.Optimizer):
                     raise TypeError(f"the moments of parameter {i} are {kinds[0]} and {kinds[1]}: a group with 32-bit states takes neither")
                 if eight:
                     self._check_names(i, state, ("exp_avg_scale", "exp_avg_sq_scale"))
+                    for name in ("exp_avg_scale", "exp_avg_sq_scale"):
+                        if state[name].shape != (state8_blocks(p.numel()),):
+                            raise ValueError(f"{name} of parameter {i} has shape {tuple(state[name].shape)}, ({state8_blocks(p.numel())},) goes with it")
                     if not (_same_layout(state["exp_avg"], p) and _same_layout(state["exp_avg_sq"], p)):
                         raise ValueError(f"the 8-bit states of parameter {i} were saved in another memory layout: their scales go with "
                                          f"256 elements that lie side by side (strides {state['exp_avg'].stride()}, the parameter's {p.stride()})")
@@ -285,9 +291,9 @@ class AdamW(torch.optim.Optimizer):
             for name, value in state_dict["state"].get(i, {}).items():
                 if name == "step":
                     self.state[p][name] = torch.as_tensor(value).to(device=p.device, dtype=torch.int64).clone()
-                elif name.endswith("_scale"):
+                elif name in ("exp_avg_scale", "exp_avg_sq_scale"):
                     self.state[p][name] = value.to(p.device).clone()
-                else:
+                elif name in ("exp_avg", "exp_avg_sq", "master"):
                     dtype = torch.float32 if group["state_bits"] == 32 else value.dtype
                     kept = torch.empty_like(p, dtype=dtype, memory_format=torch.preserve_format)
                     self.state[p][name] = kept.copy_(value)

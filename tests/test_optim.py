@@ -328,6 +328,27 @@ def test_8_bit_states_of_another_layout_are_refused(shape):
     assert wide.state[turned]["exp_avg"].stride() == turned.stride()
 
 
+def test_states_of_other_shapes_are_refused_and_further_entries_are_left_alone():
+    p, q = torch.nn.Parameter(torch.randn(8)), torch.nn.Parameter(torch.randn(4, 8))
+    for saved, kw in ((theirs_after_a_step([[p]]), {}), (with_states8(p), dict(state_bits=8))):
+        ours = optim.AdamW([q], **kw)
+        with pytest.raises(ValueError, match="shape"):
+            ours.load_state_dict(saved.state_dict())
+        assert not ours.state
+    w = torch.nn.Parameter(torch.randn(4, 8).bfloat16())
+    ours = optim.AdamW([w], master_weights=True)
+    ours.state[w].update(ours._new_state(w, ours.param_groups[0], torch.tensor(1)))
+    state = ours.state_dict()
+    with pytest.raises(ValueError, match="shape"):
+        ours.load_state_dict({**state, "state": {0: {**state["state"][0], "master": torch.zeros(8)}}})
+    eight = with_states8(q).state_dict()
+    with pytest.raises(ValueError, match="exp_avg_scale"):
+        optim.AdamW([q], state_bits=8).load_state_dict({**eight, "state": {0: {**eight["state"][0], "exp_avg_scale": torch.zeros(2)}}})
+    # what a program keeps beside the states comes as the base class has it
+    ours.load_state_dict({**state, "state": {0: {**state["state"][0], "seen": 5, "age": torch.arange(3)}}})
+    assert ours.state[w]["seen"] == 5 and ours.state[w]["age"].shape == (3,)
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
