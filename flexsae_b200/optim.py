@@ -282,9 +282,25 @@ class AdamW(torch.optim.Optimizer):
         share their count again, and a group keeps its own value of each option that the saved one does not have.  A state
         of another rule (``maximize``, ``amsgrad``, decay added to the gradient), or with moments of other types than ``state_bits`` has, is refused, with
         nothing changed; so are 8-bit states saved from a parameter of another memory layout."""
-        state_dict = self._completed(state_dict)
-        self._check_loaded(state_dict)
-        super().load_state_dict(state_dict)
+        loaded: Dict[str, dict] = {}
+
+        def before(_, state: dict) -> dict:             # behind the hooks of the program, which may replace the state
+            state = self._completed(state)
+            self._check_loaded(state)
+            loaded.update(state)
+            return state
+
+        def after(_) -> None:                           # ahead of its hooks, which see the states as they are to be
+            self._restore(loaded)
+
+        handles = [self.register_load_state_dict_pre_hook(before), self.register_load_state_dict_post_hook(after, prepend=True)]
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for handle in handles:
+                handle.remove()
+
+    def _restore(self, state_dict: dict) -> None:
         saved_ids = [i for group in state_dict["param_groups"] for i in group["params"]]
         params = [(p, group) for group in self.param_groups for p in group["params"]]
         for i, (p, group) in zip(saved_ids, params):

@@ -349,6 +349,37 @@ def test_states_of_other_shapes_are_refused_and_further_entries_are_left_alone()
     assert ours.state[w]["seen"] == 5 and ours.state[w]["age"].shape == (3,)
 
 
+def test_hooks_around_loading_see_and_set_the_states():
+    """A hook before may replace the state, one after sees the restored states and may change them."""
+    p, q = torch.nn.Parameter(torch.randn(5, 8).bfloat16()), torch.nn.Parameter(torch.randn(8))
+    theirs = theirs_after_a_step([[p], [q]])
+    ours = optim.AdamW([{"params": [p], "master_weights": True}, {"params": [q]}])
+    seen = []
+
+    def before(opt, state):
+        assert opt is ours
+        seven = {**state["state"][0], "exp_avg": torch.full((5, 8), 7.0)}
+        return {"state": {**state["state"], 0: seven}, "param_groups": [{**g, "lr": 0.5} for g in state["param_groups"]]}
+
+    def after(opt):
+        seen.append({name: x.dtype for name, x in opt.state[p].items()})
+        opt.state[q]["exp_avg"] = torch.full((8,), 9.0)
+
+    handles = [ours.register_load_state_dict_pre_hook(before), ours.register_load_state_dict_post_hook(after)]
+    ours.load_state_dict(theirs.state_dict())
+    assert seen == [{"step": torch.int64, "exp_avg": torch.float32, "exp_avg_sq": torch.float32, "master": torch.float32}]
+    assert bool((ours.state[p]["exp_avg"] == 7).all()) and bool((ours.state[q]["exp_avg"] == 9).all())
+    assert [(g["lr"], g["master_weights"]) for g in ours.param_groups] == [(0.5, True), (0.5, False)]
+    for h in handles:
+        h.remove()
+    ours.load_state_dict(theirs.state_dict())                          # and nothing of a load stays behind
+    assert len(seen) == 1 and ours.param_groups[0]["lr"] == 1e-3
+    ours.register_load_state_dict_pre_hook(lambda opt, state: {**state, "param_groups": [{**g, "maximize": True} for g in state["param_groups"]]})
+    with pytest.raises(ValueError, match="maximize"):
+        ours.load_state_dict(theirs.state_dict())
+    assert ours.param_groups[0]["lr"] == 1e-3 and not ours.param_groups[0].get("maximize")
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
