@@ -305,7 +305,9 @@ class AdamW(torch.optim.Optimizer):
         params = [(p, group) for group in self.param_groups for p in group["params"]]
         for i, (p, group) in zip(saved_ids, params):
             for name, value in state_dict["state"].get(i, {}).items():
-                if name == "step":
+                if name == "master" and p.dtype == torch.float32:
+                    del self.state[p][name]             # the parameter holds its own value
+                elif name == "step":
                     self.state[p][name] = torch.as_tensor(value).to(device=p.device, dtype=torch.int64).clone()
                 elif name in ("exp_avg_scale", "exp_avg_sq_scale"):
                     self.state[p][name] = value.to(p.device).clone()

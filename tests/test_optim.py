@@ -380,6 +380,17 @@ def test_hooks_around_loading_see_and_set_the_states():
     assert ours.param_groups[0]["lr"] == 1e-3 and not ours.param_groups[0].get("maximize")
 
 
+def test_master_copies_are_not_loaded_beside_32_bit_parameters():
+    """A state of 16-bit weights with master copies, loaded into a model that is held in 32 bits: a step refuses masters there."""
+    w = torch.nn.Parameter(torch.randn(4, 8).bfloat16())
+    sixteen = optim.AdamW([w], master_weights=True)
+    sixteen.state[w].update(sixteen._new_state(w, sixteen.param_groups[0], torch.tensor(1)))
+    q = torch.nn.Parameter(w.detach().float())
+    ours = optim.AdamW([q])
+    ours.load_state_dict(sixteen.state_dict())
+    assert sorted(ours.state[q]) == ["exp_avg", "exp_avg_sq", "step"]
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
