@@ -176,11 +176,15 @@ class AdamW(torch.optim.Optimizer):
                 self.state[p].update(self._new_state(p, group, step))
         if len(active) < len(group["params"]):      # who sits a step out keeps a count of its own
             moving = {id(self.state[p]["step"]) for p in active}
+            left: Dict[int, torch.Tensor] = {}         # together, so that they go on in one step
             for p in group["params"]:
                 if p.grad is None and self.state.get(p) and id(self.state[p]["step"]) in moving:
                     if capturing:      # every replay would copy the count again
                         raise RuntimeError("a parameter that takes part in steps outside of the captured one has no gradient in it")
-                    self.state[p]["step"] = self.state[p]["step"].clone()
+                    step = self.state[p]["step"]
+                    if id(step) not in left:
+                        left[id(step)] = step.clone()
+                    self.state[p]["step"] = left[id(step)]
         counts: Dict[int, List[torch.Tensor]] = {}
         for p in active:
             counts.setdefault(id(self.state[p]["step"]), []).append(p)

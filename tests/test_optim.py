@@ -391,6 +391,31 @@ def test_master_copies_are_not_loaded_beside_32_bit_parameters():
     assert sorted(ours.state[q]) == ["exp_avg", "exp_avg_sq", "step"]
 
 
+# ---- CPU: step counts ------------------------------------------------------------------------------------
+def let_take_part(ps, active):
+    for k, p in enumerate(ps):
+        p.grad = torch.ones_like(p) if k in active else None
+
+
+def cohorts_of(opt, ps):
+    """The positions of the parameters that step together, with their counts moved as the step would."""
+    where = {id(p): k for k, p in enumerate(ps)}
+    cohorts = opt._cohorts(opt.param_groups[0])
+    for c in cohorts:
+        opt.state[c[0]]["step"].add_(1)
+    return [[where[id(p)] for p in c] for c in cohorts]
+
+
+def test_parameters_that_sit_out_together_go_on_together():
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(5)]
+    opt = optim.AdamW(ps)
+    for active, want in (((0, 1, 2, 3, 4), [[0, 1, 2, 3, 4]]), ((0,), [[0]]), ((0, 1, 2, 3, 4), [[0], [1, 2, 3, 4]]), ((0, 1, 2), [[0], [1, 2]]),
+                         ((0, 1, 2, 3, 4), [[0], [1, 2], [3, 4]])):
+        let_take_part(ps, active)
+        assert cohorts_of(opt, ps) == want
+    assert [int(opt.state[p]["step"]) for p in ps] == [5, 4, 4, 3, 3]
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
