@@ -216,7 +216,9 @@ class AdamW(torch.optim.Optimizer):
         kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
                   masters=masters if any(t is not None for t in masters) else None, norm=self.norm, max_norm=self.max_norm)
         if group["state_bits"] == 8:
-            seed = (group["seed"] + 0x9E3779B9 * index) % 2 ** 32      # groups of one seed round independently
+            # groups of one seed, and cohorts of a group at the same count, round independently
+            place = next(k for k, p in enumerate(group["params"]) if p is ps[0])
+            seed = (group["seed"] + 0x9E3779B9 * index + 0x85EBCA6B * place) % 2 ** 32
             adamw8_step(ps, grads, column("exp_avg"), column("exp_avg_scale"), column("exp_avg_sq"), column("exp_avg_sq_scale"),
                         states[0]["step"], seed=seed, **kw)
         else:

@@ -416,6 +416,32 @@ def test_parameters_that_sit_out_together_go_on_together():
     assert [int(opt.state[p]["step"]) for p in ps] == [5, 4, 4, 3, 3]
 
 
+def test_cohorts_of_a_group_round_independently(monkeypatch):
+    """Parameters that stand at the same count, but step in different calls, are both first in their lists: the random bits of
+    those calls need different seeds, and the bits of a parameter that is first in its group those of the group's seed."""
+    calls = []
+    monkeypatch.setattr(optim, "adamw8_step", lambda ps, *a, seed, **kw: calls.append((tuple(id(p) for p in ps), seed)) or a[-1].add_(1))
+    ps = [torch.nn.Parameter(torch.ones(3)) for _ in range(4)]
+    opt = optim.AdamW(ps, state_bits=8, seed=2 ** 32 - 1)
+    first, where = 2 ** 32 - 1, [id(p) for p in ps]
+    let_take_part(ps, (0, 1, 2, 3))
+    opt.step()
+    assert calls == [(tuple(where), first)]
+    for active in ((1, 2, 3), (0, 2, 3), (0, 1, 3), (0, 1, 2)):
+        let_take_part(ps, active)
+        opt.step()
+    assert len({int(opt.state[p]["step"]) for p in ps}) == 1             # each sat out once: apart, at the same count
+    calls.clear()
+    let_take_part(ps, (0, 1, 2, 3))
+    opt.step()
+    assert sorted(c[0] for c in calls) == sorted((i,) for i in where)
+    seeds = {c[0][0]: c[1] for c in calls}
+    assert len(set(seeds.values())) == 4 and seeds[where[0]] == first and all(0 <= x < 2 ** 32 for x in seeds.values())
+    calls.clear()
+    opt.step()
+    assert {c[0][0]: c[1] for c in calls} == seeds                     # a parameter keeps its own
+
+
 # ---- GPU: helpers ---------------------------------------------------------------------------------------
 def f64(t):
     return t.detach().double().cpu().numpy()
