@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) a
       pp = fmaf(p[j], p[j], pp);
     }
     const float2 dots = team_sum2(gp, pp, part[0], team);
-    const float along = dots.y > 0.0f ? dots.x / dots.y : 0.0f;
+    const float along = dots.y == 0.0f ? 0.0f : dots.x / dots.y;    // a NaN passes
     float len = 0.0f;
 #pragma unroll
     for (int j = 0; j < 8; j++) g[j] -= along * p[j];
@@ -153,7 +153,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) a
 #pragma unroll
     for (int j = 0; j < 8; j++) len = fmaf(p[j], p[j], len);
     len = team_sum2(len, 0.0f, part[1], team).x;
-    const float scale = len > 0.0f ? 1.0f / sqrtf(len) : 1.0f;      // a row of zeros stays one
+    const float scale = len == 0.0f ? 1.0f : 1.0f / sqrtf(len);     // a row of zeros has no length to divide by
 #pragma unroll
     for (int j = 0; j < 8; j++) p[j] *= scale;
     row_store<MODE, P>(t.param, begin, n, lane, team, p2);

@@ -24,13 +24,13 @@ def adamw(p, g, m, v, t: int, lr: float, betas=(0.9, 0.999), eps: float = 1e-8, 
     g = g * clip
     if unit_rows:
         square = np.sum(p * p, axis=1, keepdims=True)
-        g = g - np.divide(np.sum(g * p, axis=1, keepdims=True), square, out=np.zeros_like(square), where=square > 0) * p
+        g = g - np.divide(np.sum(g * p, axis=1, keepdims=True), square, out=np.zeros_like(square), where=square != 0) * p
     m = betas[0] * m + (1 - betas[0]) * g
     v = betas[1] * v + (1 - betas[1]) * g * g
     p = p * (1 - lr * weight_decay) - lr / (1 - betas[0] ** t) * m / (np.sqrt(v) / np.sqrt(1 - betas[1] ** t) + eps)
     if unit_rows:
         length = np.sqrt(np.sum(p * p, axis=1, keepdims=True))
-        p = np.divide(p, length, out=p.copy(), where=length > 0)
+        p = np.divide(p, length, out=p.copy(), where=length != 0)
     return p, m, v
 
 

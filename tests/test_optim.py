@@ -1019,6 +1019,46 @@ def test_unit_rows_of_several_decoders_and_zero_rows():
         optim.adamw_unit_rows_step(*[[t] for t in y[:4]], step, lr=1e-3)
 
 
+ROW_KERNELS = [5, 8, 40, 256, 257, 640, 777, 2301, 2304, 5640, 7168, 8192]      # row lengths of every way to read a row
+
+
+def test_oracle_keeps_nothing_finite_beside_a_nan_in_a_row():
+    w = np.ones((3, 4)) / 2
+    g = np.ones((3, 4))
+    w[0, 1], w[1], g[1, 2] = np.nan, 0, np.nan
+    p, m, _ = orc.adamw(w, g, 0 * g, 0 * g, 1, 1e-2, unit_rows=True)
+    assert np.isnan(p[:2]).all() and np.isfinite(p[2]).all() and np.isnan(m[0]).all() and np.isnan(m[1]).sum() == 1
+
+
+@gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", KINDS)
+@pytest.mark.parametrize("D", ROW_KERNELS)
+def test_unit_rows_nonfinite_values_reach_their_row(dtype, grad_dtype, master, D):
+    """A NaN or an infinity in a row's parameter or gradient makes the row's length one, so no element of the row stays a number."""
+    F = 9
+    x = make((F, D), dtype, D, master, grad_dtype, spread=False)
+    w = x[4] if master else x[0]
+    w.copy_(w.float() / w.float().norm(dim=1, keepdim=True))
+    w[0, D // 2], w[2, D - 1], w[6] = math.nan, math.inf, 0
+    x[1][4, 0], x[1][6, D // 2], x[1][7, D - 1] = math.inf, math.nan, -math.inf
+    if master:
+        x[0].copy_(w)
+    b = [f64(w), f64(x[1]), f64(x[2]), f64(x[3])]
+    with np.errstate(all="ignore"):
+        want = orc.adamw(*b, 21, 1e-3, unit_rows=True)
+    optim.adamw_unit_rows_step(*[[t] for t in x[:4]], steps_in(20), lr=1e-3, masters=[x[4]] if master else None)
+    hit = np.array([0, 2, 4, 6, 7])
+    assert np.isnan(want[0][hit]).all()
+    for got in (x[0], x[4]) if master else (x[0],):
+        assert np.array_equal(np.isnan(f64(got)), np.isnan(want[0]))
+    assert np.array_equal(np.isfinite(f64(x[2])), np.isfinite(want[1]))
+    clean = [1, 3, 5, 8]
+    ep, em, ev = rows_bounds([a[clean] for a in b], [a[clean] for a in want], 21, 1e-3, 1.0)
+    check_params(x[0][clean], x[4][clean] if master else None, want[0][clean], ep, dtype)
+    close(x[2][clean], want[1][clean], em, "m")
+    close(x[3][clean], want[2][clean], ev, "v")
+
+
 # ---- GPU: streams, graphs, versions --------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
