@@ -1059,6 +1059,42 @@ def test_unit_rows_nonfinite_values_reach_their_row(dtype, grad_dtype, master, D
     close(x[3][clean], want[2][clean], ev, "v")
 
 
+@gpu
+@pytest.mark.parametrize("dtype,grad_dtype,master", [k for k in KINDS if k[0] != torch.float16 or k[2]])
+@pytest.mark.parametrize("D", ROW_KERNELS)
+def test_unit_rows_of_any_length(dtype, grad_dtype, master, D):
+    """Rows from 2^-55 to 2^64 long are stepped like others (at 2^-54, 8192 squares lose at most 8192 * 2^-150 = 2^-137 of a sum of
+    2^-108).  Shorter ones count as zeros, so that a new row is off by the old one, divided by its length; without a gradient
+    they only decay, to two roundings.  Longer ones are left as they were."""
+    lengths = [1.0, 2.0 ** 63, 1e12, 1e-8, 2.0 ** -54, 2.0 ** -54, 1e-25, 1e-38, 1e-25, 2.0 ** 66, 1e25, 1e37, 1e37]
+    F, still, short, long = len(lengths), [5, 8, 12], [6, 7, 8], [9, 10, 11, 12]
+    x = make((F, D), dtype, D + 1, master, grad_dtype, spread=False)
+    w = x[4] if master else x[0]
+    r = torch.nn.functional.normalize(torch.randn(F, D, dtype=torch.float64, generator=torch.Generator().manual_seed(D)), dim=1)
+    w.copy_(r * torch.tensor(lengths, dtype=torch.float64)[:, None])
+    if master:
+        x[0].copy_(w)
+    for k in (1, 2):
+        x[k][still] = 0
+    before = [t.clone() for t in x if t is not None]
+    b = [f64(w), f64(x[1]), f64(x[2]), f64(x[3])]
+    old = np.abs(b[0])
+    b[0][short] = 0
+    want = list(orc.adamw(*b, 21, 1e-3, unit_rows=True))
+    optim.adamw_unit_rows_step(*[[t] for t in x[:4]], steps_in(20), lr=1e-3, masters=[x[4]] if master else None)
+    for got, was in zip([t for t in x if t is not None], before):
+        assert torch.equal(got[long], was[long])
+    ep, em, ev = rows_bounds(b, want, 21, 1e-3, 1.0)
+    new = -1e-3 / (1 - 0.9 ** 21) * want[1] / (np.sqrt(want[2]) / math.sqrt(1 - 0.999 ** 21) + 1e-8)
+    ep[6:8] += old[6:8] / np.sqrt(np.sum(new[6:8] ** 2, axis=1, keepdims=True))
+    want[0][8] = f64(before[-1] if master else before[0])[8] * (1 - 1e-3 * 0.01)
+    ep[8] = 4 * U * old[8]
+    rows = list(range(9))
+    check_params(x[0][rows], x[4][rows] if master else None, want[0][rows], ep[rows], dtype)
+    close(x[2][rows], want[1][rows], em[rows], "m")
+    close(x[3][rows], want[2][rows], ev[rows], "v")
+
+
 # ---- GPU: streams, graphs, versions --------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
