@@ -480,6 +480,9 @@ __global__ void __launch_bounds__(kAdamw8Threads, sizeof(P) == 4 || sizeof(G) ==
 constexpr int64_t kOptMaxTensors = 1 << 16;
 constexpr int64_t kOptMaxNumel = 1ll << 38;
 constexpr unsigned long long kOptMaxChunks = 1ull << 30;
+// Elements of a list in all (a tensor may be in it many times): fewer than 2^30 chunks, so a launch takes as many tensors as it
+// has room for, which the workspace counts on.
+constexpr int64_t kNormMaxElements = 1ll << 42;
 // A stretch of memory that a step reads or writes.
 struct Stretch {
   uintptr_t begin, end;
@@ -680,7 +683,8 @@ extern "C" {
 
 int flexsae_grad_norm_workspace_bytes(int64_t n, int64_t elements, size_t* bytes) {
   if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
-  if (elements < 0 || !bytes) return fail(FLEXSAE_EINVAL, "%lld elements, or null pointer", (long long)elements);
+  if (elements < 0 || elements > kNormMaxElements || !bytes)
+    return fail(FLEXSAE_EINVAL, "%lld elements outside [0, 2^42], or null pointer", (long long)elements);
   *bytes = n <= kSmallBatch && elements <= kNormSmall ? 0 : (size_t)((n + kLargeBatch - 1) / kLargeBatch + 1) * kNormGrid * sizeof(double);
   return 0;
 }
@@ -713,7 +717,6 @@ int flexsae_grad_norm(const void* const* grads_host, const int64_t* numel_host, 
     for (; i < n && b.count < most; i++) {
       const unsigned long long c = ((unsigned long long)numel_host[i] + chunk - 1) / chunk;
       if (c == 0) continue;
-      if (b.count && chunks + c > kOptMaxChunks) break;
       chunks += c;
       b.grad[b.count] = grads_host[i];
       b.numel[b.count] = numel_host[i];

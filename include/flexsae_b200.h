@@ -327,7 +327,7 @@ typedef struct flexsae_optim_tensor {
 /*
  * norm_out[0] = sqrt(sum of squares over all n gradients), float32.  Squares are added in 64 bits in a
  * fixed order, so the result is the same bits every time and finite whenever it fits.  grads_host,
- * numel_host and dtypes_host are host arrays of n entries; an empty list has norm 0.  Up to 2^18 elements in
+ * numel_host and dtypes_host are host arrays of n entries, of at most 2^42 elements in all; an empty list has norm 0.  Up to 2^18 elements in
  * at most 32 tensors need no workspace (NULL, 0 bytes): flexsae_grad_norm_workspace_bytes answers what a
  * list of n tensors with that many elements in all needs.
  */

@@ -191,6 +191,20 @@ def test_norm_entry_refuses_before_any_launch():
     assert lib.flexsae_grad_norm(None, None, None, 2, 512, 1024, need, None) == -1
 
 
+def test_norm_of_more_elements_than_its_workspace_counts_on_is_refused():
+    """A tensor may be given many times: 256 of 2^36.4 elements (all of a GPU's memory, once) filled three launches' partial sums
+    where the workspace holds two.  Lists of up to 2^42 elements in all need one launch for every 256 tensors."""
+    lib = nv.load()
+    size = ctypes.c_size_t()
+    assert lib.flexsae_grad_norm_workspace_bytes(1 << 16, 1 << 42, ctypes.byref(size)) == 0
+    need = size.value
+    assert lib.flexsae_grad_norm_workspace_bytes(256, (1 << 42) + 1, ctypes.byref(size)) == -1
+    n, numel = 256, 90_000_000_000
+    rc = lib.flexsae_grad_norm((ctypes.c_void_p * n)(*[1 << 20] * n), (ctypes.c_int64 * n)(*[numel] * n), (ctypes.c_int32 * n)(*[nv.F16] * n), n, 512,
+                               1024, need, None)
+    assert rc == -1 and "elements" in lib.flexsae_last_error().decode()
+
+
 def test_python_entries_need_cuda_tensors():
     p, step = torch.zeros(8), torch.zeros((), dtype=torch.int64)
     with pytest.raises(RuntimeError, match="CUDA"):
