@@ -559,21 +559,26 @@ static int check_overlap(Stretch* s, int64_t n) {
   uintptr_t end = 0, end_written = 0;
   for (int64_t i = 0; i < n; i++) {
     if (s[i].begin < end_written || (s[i].written && s[i].begin < end))
-      return fail(FLEXSAE_EINVAL, "a tensor is given twice, or two of the tensors overlap in memory");
+      return fail(FLEXSAE_EINVAL, "a tensor is given twice, or two of the tensors (or one and the step word, lr or norm) overlap in memory");
     end = std::max(end, s[i].end);
     if (s[i].written) end_written = std::max(end_written, s[i].end);
   }
   return 0;
 }
 
-static int check_tensors(const flexsae_optim_tensor* t, int64_t n, int state_bits, bool rows) {
+static int check_tensors(const flexsae_optim_tensor* t, int64_t n, int state_bits, bool rows, const int64_t* step, const float* lr_device,
+                         const float* norm) {
   if (n < 0 || n > kOptMaxTensors) return fail(FLEXSAE_EINVAL, "%lld tensors, between 0 and %lld are supported", (long long)n, (long long)kOptMaxTensors);
-  if (n == 0) return 0;
-  if (!t) return fail(FLEXSAE_EINVAL, "null pointer argument: tensors");
-  Stretch few[7 * kSmallBatch];
-  Stretch* all = n <= kSmallBatch ? few : new (std::nothrow) Stretch[7 * n];
+  if (n > 0 && !t) return fail(FLEXSAE_EINVAL, "null pointer argument: tensors");
+  Stretch few[7 * kSmallBatch + 3];
+  Stretch* all = n <= kSmallBatch ? few : new (std::nothrow) Stretch[7 * n + 3];
   if (!all) return fail(FLEXSAE_EINVAL, "out of host memory");
   int64_t used = 0;
+  const struct { const void* p; size_t bytes; bool written; } words[] = {{step, 8, true}, {lr_device, 4, false}, {norm, 4, false}};
+  for (const auto& w : words) {
+    const uintptr_t b = reinterpret_cast<uintptr_t>(w.p);
+    if (w.p) all[used++] = Stretch{b, b + w.bytes, w.written};
+  }
   int rc = 0;
   for (int64_t i = 0; i < n && rc == 0; i++) {
     int k = 0;
@@ -769,7 +774,7 @@ int flexsae_adamw_step(const flexsae_optim_tensor* tensors_host, int64_t n, int 
   t_launches = 0;
   if (state_bits != 32 && state_bits != 8) return fail(FLEXSAE_EINVAL, "states of %d bits: 32 and 8 are supported", state_bits);
   if (int rc = check_scalars(step, lr, beta1, beta2, eps, weight_decay, norm, max_norm)) return rc;
-  if (int rc = check_tensors(tensors_host, n, state_bits, false)) return rc;
+  if (int rc = check_tensors(tensors_host, n, state_bits, false, step, lr_device, norm)) return rc;
   return adamw_impl(tensors_host, n, state_bits,
                     make_scalars(step, lr, lr_device, beta1, beta2, eps, weight_decay, norm, max_norm, seed),
                     reinterpret_cast<cudaStream_t>(stream));
@@ -780,7 +785,7 @@ int flexsae_adamw_unit_rows_step(const flexsae_optim_tensor* tensors_host, int64
                                  const float* norm, double max_norm, void* stream) {
   t_launches = 0;
   if (int rc = check_scalars(step, lr, beta1, beta2, eps, weight_decay, norm, max_norm)) return rc;
-  if (int rc = check_tensors(tensors_host, n, 32, true)) return rc;
+  if (int rc = check_tensors(tensors_host, n, 32, true, step, lr_device, norm)) return rc;
   const OptScalars s = make_scalars(step, lr, lr_device, beta1, beta2, eps, weight_decay, norm, max_norm, 0);
   cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
   int64_t last = -1;

@@ -77,7 +77,7 @@ def adamw_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, exp_avg_sq
     16-bit parameter loses changes below half its spacing).  ``lr``: a number, or a float32 tensor on the
     device (which a captured graph follows).  ``norm``: the norm of all gradients, from ``grad_norm``;
     with it c = min(1, max_norm / (norm + 1e-6)), and a norm that is not finite leaves everything as it
-    was.  A tensor given twice, or tensors that overlap, are refused."""
+    was.  A tensor given twice, or tensors that overlap (``step``, ``lr`` and ``norm`` among them), are refused."""
     _step(_ADAMW, params, grads, exp_avgs, None, exp_avg_sqs, None, masters, step, lr, betas, eps, weight_decay, norm, max_norm)
 
 

@@ -308,7 +308,8 @@ int flexsae_loss_fwd_static_scratch(int kind, const int64_t* indices, const void
  * A step takes a host array of tensors.  All pointers in it are device pointers, aligned to their
  * elements; aligned to eight elements (32, 16 or 8 bytes) they are faster.  Elements are taken in memory order, so
  * the tensors of one entry have the same layout.  An entry with numel 0 is passed over.  Memory that
- * a step writes must not overlap anything else in its list: this is checked, and refused.
+ * a step writes must not overlap anything else that it is given (the step word, lr_device and norm among it): this is
+ * checked, and refused.
  */
 typedef struct flexsae_optim_tensor {
   void* param;               /* updated in place */

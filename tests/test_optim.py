@@ -161,6 +161,16 @@ def test_step_entries_refuse_before_any_launch(kw, text):
     assert rc < 0 and text in err, (rc, err)
 
 
+@pytest.mark.parametrize("kw", [dict(step=1 << 20), dict(step=(2 << 20) + 8), dict(step=(4 << 20) + 2040), dict(norm=(1 << 20) + 4), dict(lr_dev=3 << 20),
+                                dict(norm=512), dict(lr_dev=516), dict(bits=8, step=5 << 20), dict(n=40, norm=(4 << 20) + (30 << 24))])
+@pytest.mark.parametrize("rows", [False, True])
+def test_a_step_word_norm_or_learning_rate_inside_a_tensor_is_refused(kw, rows):
+    """A step reads them while it writes the tensors, and writes the step word while it reads the gradients."""
+    if not (rows and "bits" in kw):
+        rc, err = _entry(rows=rows, **kw)
+        assert rc < 0 and "overlap" in err, (rc, err)
+
+
 def test_norm_entry_refuses_before_any_launch():
     lib = nv.load()
     size = ctypes.c_size_t()
