@@ -240,8 +240,10 @@ long run_step(PyObject* const* a) {
     written(params[i]);
     written(m[i]);
     written(v[i]);
+    if (kind == kAdamw8) written(ms[i]), written(vs[i]);
     if (with_masters && masters[i].defined()) written(masters[i]);
   }
+  written(step);
   return g.launches();
 }
 

@@ -1339,6 +1339,17 @@ def test_autograd_sees_that_a_parameter_changed():
         loss.backward()
 
 
+@gpu
+def test_every_tensor_that_a_step_writes_counts_a_version():
+    p, g, _, _, w = make((16, 32), torch.bfloat16, 3, master=True)
+    m, v = (torch.zeros(16, 32, device="cuda").to(d) for d in optim.STATE8_DTYPES)
+    scales, step, norm = [torch.zeros(2, device="cuda") for _ in range(2)], steps_in(0), optim.grad_norm([g])
+    tensors = [p, w, m, v, *scales, step, g, norm]
+    before = [t._version for t in tensors]
+    optim.adamw8_step([p], [g], [m], [scales[0]], [v], [scales[1]], step, lr=1e-3, masters=[w], norm=norm)
+    assert [t._version - k for t, k in zip(tensors, before)] == [1] * 7 + [0] * 2
+
+
 # ---- GPU: the optimizer class, and a training run -----------------------------------------------------------
 def make_sae(F, D, dtype, seed=0):
     g = torch.Generator().manual_seed(seed)
