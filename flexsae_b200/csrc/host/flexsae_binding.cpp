@@ -86,11 +86,17 @@ bool same_layout(const at::Tensor& a, const at::Tensor& b) {
 
 bool dense(const at::Tensor& t) { return t.numel() == 0 || t.is_contiguous() || t.unsafeGetTensorImpl()->is_non_overlapping_and_dense(); }
 
+// A view that stands for the negated values of its memory is not what a kernel would read.
+void check_as_stored(const char* name, const at::Tensor& t) {
+  if (t.is_neg()) refuse(PyExc_ValueError, name, " must not be a lazily negated view");
+}
+
 void check_one(const char* name, const at::Tensor& t, const at::Tensor& p, at::ScalarType type) {
   if (t.scalar_type() != type) refuse(PyExc_TypeError, name, " must be ", type, ", got ", t.scalar_type());
   if (t.device() != p.device()) refuse(PyExc_RuntimeError, "a tensor in ", name, " is on ", t.device(), ", the parameters are on ", p.device());
   if (!t.sizes().equals(p.sizes()) || !same_layout(t, p))
     refuse(PyExc_ValueError, "a tensor in ", name, " has shape ", t.sizes(), " and strides ", t.strides(), ", its parameter ", p.sizes(), " and ", p.strides());
+  check_as_stored(name, t);
 }
 
 void check_count(const char* name, const List& list, const List& params) {
@@ -103,6 +109,7 @@ void check_scales(const char* name, const at::Tensor& t, const at::Tensor& p) {
   if (t.device() != p.device()) refuse(PyExc_RuntimeError, "a tensor in ", name, " is on ", t.device(), ", the parameters are on ", p.device());
   if (t.dim() != 1 || t.size(0) != blocks || !t.is_contiguous())
     refuse(PyExc_ValueError, name, " of ", p.numel(), " elements is contiguous float32 [", blocks, "], got ", t.sizes());
+  check_as_stored(name, t);
 }
 
 // A number on the device.
@@ -111,6 +118,7 @@ const at::Tensor& word(const char* name, PyObject* o, at::ScalarType type, const
   const at::Tensor& t = THPVariable_Unpack(o);
   if (t.scalar_type() != type) refuse(PyExc_TypeError, name, " must be ", type, ", got ", t.scalar_type());
   if (t.device() != dev) refuse(PyExc_RuntimeError, name, " is on ", t.device(), ", the parameters are on ", dev);
+  check_as_stored(name, t);
   return t;
 }
 
@@ -173,6 +181,7 @@ long run_step(PyObject* const* a) {
       refuse(PyExc_RuntimeError, "parameters and gradients must be on one device, got ", p.device(), " and ", grad.device(), " beside ", dev);
     if (!grad.sizes().equals(p.sizes())) refuse(PyExc_ValueError, "a gradient has shape ", grad.sizes(), ", its parameter ", p.sizes());
     if (!dense(p)) refuse(PyExc_ValueError, "a parameter of shape ", p.sizes(), " with strides ", p.strides(), " does not fill its memory");
+    check_as_stored("params", p);
     if (kind == kUnitRows && (p.dim() != 2 || !p.is_contiguous()))
       refuse(PyExc_ValueError, "unit rows need a contiguous [F, D] parameter, got ", p.sizes(), " with strides ", p.strides());
     check_one("exp_avgs", m[i], p, type_m);
@@ -210,7 +219,7 @@ long run_step(PyObject* const* a) {
   for (size_t i = 0; i < n; i++) {
     const at::Tensor& p = params[i];
     const at::Tensor* grad = &grads[i];
-    if (!same_layout(*grad, p)) {
+    if (!same_layout(*grad, p) || grad->is_neg()) {
       copies.push_back(at::empty_like(p, p.options().dtype(grad->scalar_type()).requires_grad(false)).copy_(grad->detach()));
       grad = &copies.back();
     }

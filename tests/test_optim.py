@@ -699,6 +699,24 @@ def test_layouts_transposed_parameters_and_foreign_gradients():
 
 
 @gpu
+def test_lazily_negated_views():
+    """A view whose memory holds the negated values (torch keeps such for parts of conjugates): a gradient is read as what it stands for,
+    what a step writes or reads as a word is refused."""
+    x = make((48, 80), torch.float32, 8)
+    y, step = [t.clone() for t in x[:4]], steps_in(0)
+    negated = torch._neg_view(-x[1])
+    assert torch.equal(negated, x[1]) and negated.is_neg()
+    optim.adamw_step([x[0]], [negated], [x[2]], [x[3]], step, lr=1e-3)
+    optim.adamw_step(*[[t] for t in y], steps_in(0), lr=1e-3)
+    assert torch.equal(x[0], y[0]) and torch.equal(x[2], y[2])
+    norm = torch.ones((), device="cuda")
+    for k, kw in ((0, {}), (2, {}), (3, {}), (None, dict(norm=torch._neg_view(norm))), (None, dict(lr=torch._neg_view(norm)))):
+        args = [[torch._neg_view(t) if i == k else t] for i, t in enumerate(y)]
+        with pytest.raises(ValueError, match="negated"):
+            optim.adamw_step(*args, step, **{**dict(lr=1e-3), **kw})
+
+
+@gpu
 def test_python_refusals_on_cuda_tensors():
     p, g, m, v, _ = make((16, 32), torch.bfloat16, 9)
     step = steps_in(0)
