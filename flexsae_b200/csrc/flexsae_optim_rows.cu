@@ -117,7 +117,7 @@ constexpr float kLeastSquare = 0x1p-110f;
 // parameters and gradients up to 896 (72), have the next row's loads under way: 60 M bf16 in rows of 5120 / 7168 take 215 /
 // 206 us with them and 297 / 262 without; fp32 in rows of 7168 would spill (353 and 295).
 template <RowMode MODE, typename P, typename G, bool MASTER, int MOST>
-__global__ void __launch_bounds__(MOST, MOST <= 288 ? 4 : MOST <= 576 ? 2 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
+__global__ void __launch_bounds__(MOST, MOST <= 576 ? 2 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
   using W = typename std::conditional<MASTER, float, P>::type;      // type that holds the parameter's value
   __shared__ float2 part[2][32];
   const OptTensor& t = a.t;
@@ -180,9 +180,7 @@ constexpr int kGroupedFrom = 640;
 
 template <RowMode MODE, typename P, typename G, bool M>
 static cudaError_t launch_mode(const RowArgs& a, int threads, cudaStream_t st) {
-  auto kernel = threads <= 288   ? adamw_unit_rows_kernel<MODE, P, G, M, 288>
-                : threads <= 576 ? adamw_unit_rows_kernel<MODE, P, G, M, 576>
-                                 : adamw_unit_rows_kernel<MODE, P, G, M, 1024>;
+  auto kernel = threads <= 576 ? adamw_unit_rows_kernel<MODE, P, G, M, 576> : adamw_unit_rows_kernel<MODE, P, G, M, 1024>;
   if constexpr (MODE == kWholeRows) {
     if (threads > 576 && threads <= 704) kernel = adamw_unit_rows_kernel<MODE, P, G, M, 704>;
     if constexpr (sizeof(P) == 2 && sizeof(G) == 2 && !M)
