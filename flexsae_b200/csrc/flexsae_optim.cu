@@ -152,7 +152,8 @@ __global__ void __cluster_dims__(kNormCluster, 1, 1) __launch_bounds__(kNormClus
 }
 
 // ---- AdamW, 32-bit states -----------------------------------------------------------------------------
-// Bound by HBM: 302 M bf16 parameters in 1.03 ms (99 % of the measured copy rate), 268 M fp32 in 1.13 ms (102 %).
+// Bound by HBM: 302 M bf16 parameters in 1.03 ms (99 % of the measured copy rate), 268 M fp32 in 1.13 ms (102 %); not
+// aligned to eight elements, where single elements are moved, 100 M bf16 take 446 instead of 340 us and fp32 448 instead of 421.
 constexpr int kAdamwThreads = 128, kAdamw8Threads = 256;
 
 // The chunks of all tensors (a unit for every one of a CTA's warps) are dealt out to the CTAs in turn.  Step is told about
@@ -284,7 +285,9 @@ __device__ __forceinline__ unsigned top_bytes(unsigned a, unsigned b, unsigned c
   return __byte_perm(__byte_perm(a, b, 0x0073), __byte_perm(c, d, 0x0073), 0x5410);
 }
 
-// The step, to the same bits as Adamw8Step, for a unit that is cut off, not aligned, or holds an infinity or NaN, which
+// The step, to the same bits as Adamw8Step, for a unit that is cut off, not aligned (all of a tensor's units, if one of its
+// pointers is not: 100 M bf16 parameters 516 instead of 180 us, since every access moves one element, every element has a hash
+// of its own and no unit is on its way while another is worked on), or holds an infinity or NaN, which
 // keep to their own elements: the scale is that of the others (e4m3 has no infinity: a NaN stands for it).  With an eps below kLeastEps, for which the
 // approximate root is not good enough, all units come here.
 template <typename P, typename G, bool MASTER>
@@ -338,7 +341,7 @@ __device__ __forceinline__ void adamw8_part(const OptScalars& s, const OptCoefs&
 
 // The 32-bit form has 22 bytes of traffic per element to hide its arithmetic behind, this one 10: at HBM
 // speed an SM may spend about 49 instructions on an element; the kernel takes 43.5, and 302 M bf16 parameters
-// 0.57 ms, 82 % of the HBM rate (0.78 ms and 96 % with fp32 parameters).  So the arithmetic is in packed pairs,
+// 0.59 ms, 79 % of the HBM rate (0.78 ms and 96 % with fp32 parameters).  So the arithmetic is in packed pairs,
 // root and reciprocal are the approximate ones (2 u each; they only reach the parameter), the codes are
 // formed in the top byte of a word, where shift and random bits are one addition, one hash serves a
 // pair of elements, and a warp's next unit is on its way while it works on one.
@@ -452,8 +455,6 @@ struct Adamw8Step {
     Raw8<unsigned char> cm, cv;
     cm.w = make_uint2(top_bytes(qm[0], qm[1], qm[2], qm[3]), top_bytes(qm[4], qm[5], qm[6], qm[7]));
     cv.w = make_uint2(top_bytes(qv[0], qv[1], qv[2], qv[3]), top_bytes(qv[4], qv[5], qv[6], qv[7]));
-    // The floor of v (see code_e5m2) on the finished codes, four at a time: 0 becomes 1, since a byte of at most 0x7f has
-    // its top bit set after 0x7f was added unless it is 0.
     cm.store(at.m + e);
     cv.store(at.v + e);
     if (threadIdx.x % 32 == 0) {

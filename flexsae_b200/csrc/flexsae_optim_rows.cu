@@ -3,7 +3,7 @@
 //
 // A team of threads holds a row, eight elements each, so it stays in registers between its three uses: the CTA, or,
 // for rows of up to 256 elements, a warp or a power-of-two part of one (no barrier then).  A row is read and written
-// once; 65536 rows of 2304 bf16 take 0.51 ms, 99 % of the HBM rate.
+// once; 65536 rows of 2304 bf16 take 0.52 ms, 98 % of the HBM rate.
 #include <type_traits>
 
 #include "flexsae_optim.cuh"
@@ -111,11 +111,14 @@ struct RowRaw {
 // rows again, scaled, is a branch in the loop: 131072 rows of 777 bf16 605 instead of 484 us, 29296 of 4096 475 instead of 406.
 constexpr float kLeastSquare = 0x1p-110f;
 
-// MOST: threads of a CTA at most.  The registers of a thread (56) are set so that an SM holds four CTAs of up to 288 threads
-// or two of up to 576: 65536 rows of 2304 bf16 take 541 us with four CTAs and 556 with three (a fifth spills: 767 us).
-// Where an SM holds one CTA, nothing covers its waits, so whole rows of up to 704 threads (88 registers), with 16-bit
+// MOST: threads of a CTA at most.  The registers of a thread (56) are set so that an SM holds two CTAs of up to 576 threads, four
+// of up to 288 or nine of 128: 65536 rows of 2304 bf16 (288 threads) take 522 us with room for four or three, 559 with room for
+// five, which spills; 77319 of 776 (128 threads) 209, 225 with the registers of three.
+// Where an SM holds one CTA, nothing covers its waits, so whole rows of up to 704 threads (80 registers), with 16-bit
 // parameters and gradients up to 896 (72), have the next row's loads under way: 60 M bf16 in rows of 5120 / 7168 take 215 /
-// 206 us with them and 297 / 262 without; fp32 in rows of 7168 would spill (353 and 295).
+// 206 us with them and 292 / 260 without; fp32 in rows of 7168 would spill much (356 and 296).  Kernels that spill as they
+// are: 4 to 20 bytes in the 704 class with fp32 parameters or with fp32 gradients and masters, in the 896 class and in grouped
+// fp32 rows of up to 576 threads; 12 to 48 bytes in all kernels of strided rows.
 template <RowMode MODE, typename P, typename G, bool MASTER, int MOST>
 __global__ void __launch_bounds__(MOST, MOST <= 576 ? 2 : 1) adamw_unit_rows_kernel(const __grid_constant__ RowArgs a) {
   using W = typename std::conditional<MASTER, float, P>::type;      // type that holds the parameter's value
@@ -161,7 +164,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 576 ? 2 : 1) adamw_unit_rows_ker
 #pragma unroll
     for (int j = 0; j < 8; j++) len = fmaf(p[j], p[j], len);
     len = team_sum2(len, 0.0f, part[1], team).x;
-    const float scale = len < kLeastSquare ? 1.0f : 1.0f / sqrtf(len);
+    const float scale = len < kLeastSquare ? 1.0f : 1.0f / sqrtf(len);      // one division instead of eight: half an ulp more
     const int put = wide || len > FLT_MAX ? 0 : n;
 #pragma unroll
     for (int j = 0; j < 8; j++) p[j] *= scale;
@@ -175,7 +178,7 @@ __global__ void __launch_bounds__(MOST, MOST <= 576 ? 2 : 1) adamw_unit_rows_ker
 
 constexpr int kRowThreads = 128;      // of a CTA whose rows have a warp or less each
 // Rows that do not begin at a group of eight are read in groups from here on (their ends are accesses of
-// single elements; bf16: 77220 rows of 777 take 286 us in groups and 325 strided, 131072 of 257 311 and 271).
+// single elements; bf16: 77220 rows of 777 take 293 us in groups and 330 strided, 131072 of 257 319 and 274).
 constexpr int kGroupedFrom = 640;
 
 template <RowMode MODE, typename P, typename G, bool M>
