@@ -139,20 +139,24 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
         group = self.param_groups[-1]
         try:
-            if group["state_bits"] not in (8, 32):
-                raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
-            if not 0 <= group["seed"] < 2 ** 32:
-                raise ValueError(f"seed must be in [0, 2**32), got {group['seed']}")
-            if group["unit_rows"] and group["state_bits"] != 32:
-                raise ValueError("unit_rows goes with 32-bit states")
-            for p in group["params"]:
-                if p.dtype not in nv.DTYPE_CODES:
-                    raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
-                if group["unit_rows"] and p.dim() != 2:
-                    raise ValueError(f"unit rows need [F, D] parameters, got {tuple(p.shape)}")
+            self._check_group(group, group["params"])
         except (ValueError, TypeError):
             self.param_groups.pop()
             raise
+
+    @staticmethod
+    def _check_group(group: dict, params: Sequence[torch.Tensor]) -> None:
+        if group["state_bits"] not in (8, 32):
+            raise ValueError(f"state_bits must be 8 or 32, got {group['state_bits']}")
+        if not 0 <= group["seed"] < 2 ** 32:
+            raise ValueError(f"seed must be in [0, 2**32), got {group['seed']}")
+        if group["unit_rows"] and group["state_bits"] != 32:
+            raise ValueError("unit_rows goes with 32-bit states")
+        for p in params:
+            if p.dtype not in nv.DTYPE_CODES:
+                raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
+            if group["unit_rows"] and p.dim() != 2:
+                raise ValueError(f"unit rows need [F, D] parameters, got {tuple(p.shape)}")
 
     def _new_state(self, p: torch.Tensor, group: dict, step: torch.Tensor) -> Dict[str, torch.Tensor]:
         kinds = STATE8_DTYPES if group["state_bits"] == 8 else (torch.float32, torch.float32)
@@ -251,8 +255,12 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"the state of parameter {i} has no {', '.join(missing)}: it is not one of AdamW")
 
     def _check_loaded(self, state_dict: dict) -> None:
-        """Refuses a state that these steps would not continue: of another rule, or without the moments in the group's form."""
+        """Refuses a state that these steps would not continue: of another rule, without the moments in the group's form, or with
+        options that do not go together or with the parameters."""
+        if len(state_dict["param_groups"]) != len(self.param_groups):      # refused by the base class
+            return
         for group, mine in zip(state_dict["param_groups"], self.param_groups):
+            self._check_group(group, mine["params"])
             for name in ("maximize", "amsgrad"):
                 if group.get(name):
                     raise ValueError(f"the state was saved with {name}=True, which this optimizer does not have")

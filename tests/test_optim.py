@@ -415,6 +415,18 @@ def test_master_copies_are_not_loaded_beside_32_bit_parameters():
     assert sorted(ours.state[q]) == ["exp_avg", "exp_avg_sq", "step"]
 
 
+@pytest.mark.parametrize("theirs,ours,text", [
+    (dict(state_bits=8), dict(unit_rows=True), "unit_rows"), (dict(state_bits=16), {}, "state_bits"), (dict(seed=-1), {}, "seed"),
+    (dict(unit_rows=True), dict(shape=(8,)), "unit rows"),
+])
+def test_options_that_do_not_go_together_are_refused_at_load_too(theirs, ours, text):
+    p = torch.nn.Parameter(torch.randn(ours.get("shape", (4, 8))))
+    opt = optim.AdamW([p], lr=2e-3, **{k: v for k, v in ours.items() if k != "shape"})
+    with pytest.raises(ValueError, match=text):
+        opt.load_state_dict({"state": {}, "param_groups": [{"params": [0], "lr": 1e-3, **theirs}]})
+    assert opt.param_groups[0]["lr"] == 2e-3 and opt.param_groups[0]["state_bits"] == 32
+
+
 # ---- CPU: step counts ------------------------------------------------------------------------------------
 def let_take_part(ps, active):
     for k, p in enumerate(ps):
