@@ -107,8 +107,9 @@ struct RowRaw {
 // Sums are held in 32 bits.  A sum of squares below this has lost more than 2^-27 of itself to terms that vanished: the row, shorter
 // than 2^-55, counts as a row of zeros, which has no direction to project on and no length to divide by.  A row whose
 // squares overflow, longer than 2^64, is left as it was, with its moments: divided by an infinite length it would
-// become zeros.  (An infinity in the row or its gradient makes their product infinite or NaN, and then the row.)  Taking such
-// rows again, scaled, is a branch in the loop: 131072 rows of 777 bf16 605 instead of 484 us, 29296 of 4096 475 instead of 406.
+// become zeros.  (An infinity in the row or its gradient makes their product infinite or NaN, and then the row; so does a
+// finite gradient whose product with the row passes 2^128.)  Taking such rows again, scaled, is a branch in the
+// loop: 131072 rows of 777 bf16 605 instead of 484 us, 29296 of 4096 475 instead of 406.
 constexpr float kLeastSquare = 0x1p-110f;
 
 // MOST: threads of a CTA at most.  The registers of a thread (56) are set so that an SM holds two CTAs of up to 576 threads, four

@@ -106,7 +106,8 @@ def adamw_unit_rows_step(params: _Tensors, grads: _Tensors, exp_avgs: _Tensors, 
     gradient's component along its row is taken out first (g -= (g.w / w.w) w), and after the step
     the row is divided by its length.  A row of zeros has no direction and no length: its gradient stays whole, and where the step
     leaves it zeros it is not divided.  An infinity or NaN in a parameter or gradient reaches its row.  Sums over a row are
-    held in 32 bits: a row shorter than 2^-55 counts as zeros, one longer than 2^64 is left as it was, with its moments."""
+    held in 32 bits: a row shorter than 2^-55 counts as zeros, one longer than 2^64 is left as it was, with its moments,
+    and a gradient whose product with its row passes 2^128 counts as infinite."""
     _step(_UNIT_ROWS, params, grads, exp_avgs, None, exp_avg_sqs, None, masters, step, lr, betas, eps, weight_decay, norm, max_norm)
 
 

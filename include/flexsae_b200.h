@@ -362,7 +362,8 @@ int flexsae_adamw_step(const flexsae_optim_tensor* tensors_host, int64_t n, int 
  * the step the row is divided by its length.  A row of zeros has no direction and no length: its gradient
  * stays whole, and where the step leaves it zeros it is not divided.  An infinity or NaN reaches its row.  Sums over
  * a row are held in 32 bits: a row shorter than 2^-55 counts as zeros, one longer than 2^64 is left as it was, with
- * its moments.  One launch for every tensor; rows of up to 8192 elements.
+ * its moments, and a gradient whose product with its row passes 2^128 counts as infinite.  One launch for every tensor;
+ * rows of up to 8192 elements.
  */
 int flexsae_adamw_unit_rows_step(const flexsae_optim_tensor* tensors_host, int64_t n, int64_t* step, double lr,
                                  const float* lr_device, double beta1, double beta2, double eps, double weight_decay,

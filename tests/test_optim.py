@@ -1149,6 +1149,22 @@ def test_unit_rows_of_any_length(dtype, grad_dtype, master, D):
     close(x[3][rows], want[2][rows], ev[rows], "v")
 
 
+@gpu
+@pytest.mark.parametrize("D", ROW_KERNELS)
+def test_unit_rows_whose_product_with_the_gradient_overflows(D):
+    """Sums over a row are 32-bit: D products of 2e38 / sqrt(D) are sqrt(D) 2e38, past 2^128 from D = 3 on.  The row counts as one with
+    an infinity, its neighbours do not notice, and with a clipping factor the same gradient is an ordinary one."""
+    w = torch.full((4, D), D ** -0.5, device="cuda")
+    g = torch.randn(4, D, generator=torch.Generator().manual_seed(D)).cuda()
+    g[1] = 2e38
+    zeros = [torch.zeros(4, D, device="cuda") for _ in range(4)]
+    first, second = w.clone(), w.clone()
+    optim.adamw_unit_rows_step([first], [g], zeros[:1], zeros[1:2], steps_in(0), lr=1e-3)
+    assert bool(torch.isnan(first[1]).all()) and bool(torch.isfinite(first[[0, 2, 3]]).all())
+    optim.adamw_unit_rows_step([second], [g], zeros[2:3], zeros[3:], steps_in(0), lr=1e-3, norm=torch.tensor(1e30, device="cuda"), max_norm=1.0)
+    assert float((second.double().norm(dim=1) - 1).abs().max()) <= 16 * U
+
+
 # ---- GPU: streams, graphs, versions --------------------------------------------------------------------
 @gpu
 @pytest.mark.parametrize("bits", [32, 8])
